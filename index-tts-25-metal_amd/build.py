@@ -37,7 +37,7 @@ DEVICE_FLAGS = [
     f"-I{CSRC}",
 ]
 SOURCES = ["decode.hip", "step.hip", "step_bf16.hip", "step_batch.hip", "sampler.hip", "beam.hip", "prefill.hip", "util.hip", "runtime.hip",
-           "codec.hip", "libm_check.hip", "qwen.hip"]
+           "codec.hip", "libm_check.hip", "qwen.hip", "q4.hip"]
 # Per-file device flags.  step.hip: the persistent step kernel is scheduled with LLVM's max-ILP
 # strategy, 578.4 -> 567.9 us per step at 752 cached rows (one box, three alternating runs); the
 # same strategy made the batched GEMVs of decode.hip 9% slower, so it is not applied there.

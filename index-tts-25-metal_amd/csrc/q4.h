@@ -1,0 +1,49 @@
+// Launch arguments and launchers of the kernels on 4-bit weights and 8-bit activations (q4.hip).
+// The formats are those of include/itts_ops.h, whose entry points check what is assumed here.
+#pragma once
+#include "common.h"
+
+namespace itts {
+namespace q4 {
+
+struct NormArgs {
+    const void* x;
+    int64_t x_stride;
+    const void* residual;  // or null
+    int64_t residual_stride;
+    const void* weight;    // null: no norm
+    int weight_dtype, dtype;
+    int64_t rows, cols;
+    float eps;
+    int group;
+    void* h_out;           // or null
+    int64_t h_stride;
+    void* values;          // or null
+    int64_t values_stride;
+    int8_t* q;
+    float* scales;
+};
+hipError_t launch_rows(const NormArgs& a, hipStream_t s);
+
+struct ProductArgs {
+    const int8_t* q;
+    const float* qscales;
+    int rows;
+    const uint8_t* packed;
+    const uint16_t* wscales;
+    int n, k, group;
+    const float* bias;     // or null
+    const void* residual;  // or null
+    int64_t residual_stride;
+    bool swiglu;
+    int dtype;
+    void* out;
+    int64_t out_stride;
+};
+hipError_t launch_product(const ProductArgs& a, hipStream_t s);
+
+hipError_t launch_pack(const void* w, int64_t stride, int dtype, int n, int k, int group, void* packed, void* scales, hipStream_t s);
+hipError_t launch_unpack(const void* packed, const void* scales, int n, int k, int group, int dtype, void* out, int64_t stride, hipStream_t s);
+
+}  // namespace q4
+}  // namespace itts

@@ -1,0 +1,131 @@
+"""What the operators on 4-bit weights and 8-bit activations refuse: checked before anything is enqueued, so
+without a GPU, through itts_ops and through the C ABI."""
+import ctypes as C
+
+import pytest
+import torch
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def ops(itts):
+    import itts_ops
+
+    return itts_ops
+
+
+def weight(ops, n=20, k=130, group=64):
+    nt, kb = -(-n // 16), -(-k // 128)
+    return ops.Q4Weight(torch.zeros(nt, kb, 1024, dtype=torch.uint8), torch.zeros(nt, kb, 16, 128 // group, dtype=BF16), n, k, group)
+
+
+def refused(itts, match, fn, *args, **kw):
+    with pytest.raises(itts.InvalidArgument, match=match):
+        fn(*args, **kw)
+
+
+def test_rows_to_codes(itts, ops):
+    x, w = torch.zeros(3, 40), torch.ones(40)
+    refused(itts, "on the GPU", ops.rmsnorm_q8, x, w)
+    refused(itts, "on the GPU", ops.q8_quantize, x)
+    refused(itts, "float32, bfloat16 or float16", ops.q8_quantize, x.double())
+    refused(itts, "a matrix is wanted", ops.q8_quantize, x[0])
+    refused(itts, "next to each other", ops.q8_quantize, x.t())
+    refused(itts, "32, 64 or 128", ops.q8_quantize, x, 16)
+    refused(itts, "32, 64 or 128", ops.rmsnorm_q8, x, w, group=256)
+    refused(itts, "weight: 40", ops.rmsnorm_q8, x, w[:39])
+    refused(itts, "weight: 40", ops.rmsnorm_q8, x, torch.ones(80)[::2])
+    refused(itts, "weight: torch.float32 or float32", ops.rmsnorm_q8, x, w.bfloat16())
+    refused(itts, "residual", ops.rmsnorm_q8, x, w, residual=x[:2])
+    refused(itts, "residual", ops.rmsnorm_q8, x, w, residual=x.bfloat16())
+    refused(itts, "h:", ops.rmsnorm_q8, x, w, h=torch.zeros(3, 41))
+    refused(itts, "values:", ops.q8_quantize, x, values=torch.zeros(3, 41))
+    refused(itts, "q:", ops.q8_quantize, x, q=torch.zeros(3, 40, dtype=torch.int8))
+    refused(itts, "scales:", ops.q8_quantize, x, scales=torch.zeros(3, 2))
+
+
+def test_weights(itts, ops):
+    refused(itts, "on the GPU", ops.q4_pack, torch.zeros(3, 4))
+    refused(itts, "without rows or columns", ops.q4_pack, torch.zeros(0, 4))
+    refused(itts, "without rows or columns", ops.q4_pack, torch.zeros(4, 0))
+    refused(itts, "32, 64 or 128", ops.q4_pack, torch.zeros(3, 4), 33)
+    refused(itts, "Q4Weight", ops.q4_unpack, torch.zeros(3, 4))
+    w = weight(ops)
+    refused(itts, "on the GPU", ops.q4_unpack, w)
+    refused(itts, "dtype", ops.q4_unpack, w, torch.int8)
+    refused(itts, "out", ops.q4_unpack, w, out=torch.zeros(20, 131))
+    refused(itts, "packed codes", ops.q4_unpack, w._replace(n=33))
+    refused(itts, "packed codes", ops.q4_unpack, w._replace(packed=w.packed[:1]))
+    refused(itts, "packed codes", ops.q4_unpack, w._replace(packed=w.packed.to(torch.int8)))
+    refused(itts, "the scales", ops.q4_unpack, w._replace(group=32))
+    refused(itts, "32, 64 or 128", ops.q4_unpack, w._replace(group=48))
+
+
+def test_products(itts, ops):
+    w = weight(ops)
+    q, s = torch.zeros(3, 256, dtype=torch.int8), torch.zeros(3, 4)
+    refused(itts, "on the GPU", ops.q4_matmul, q, s, w)
+    refused(itts, "q: ", ops.q4_matmul, q[:, :128], s, w)
+    refused(itts, "q: ", ops.q4_matmul, q.float(), s, w)
+    refused(itts, "q: ", ops.q4_matmul, q[:, ::2], s, weight(ops, 20, 100))
+    refused(itts, "scales: ", ops.q4_matmul, q, s[:2], w)
+    refused(itts, "scales: ", ops.q4_matmul, q, torch.zeros(3, 2), w)
+    refused(itts, "bias", ops.q4_matmul, q, s, w, bias=torch.zeros(19))
+    refused(itts, "bias", ops.q4_matmul, q, s, w, bias=torch.zeros(20, dtype=BF16))
+    refused(itts, "residual", ops.q4_matmul, q, s, w, residual=torch.zeros(3, 19))
+    refused(itts, "residual", ops.q4_matmul, q, s, w, residual=torch.zeros(3, 20), out_dtype=BF16)
+    refused(itts, "out_dtype", ops.q4_matmul, q, s, w, out_dtype=torch.float64)
+    refused(itts, "out: ", ops.q4_matmul, q, s, w, out=torch.zeros(3, 21))
+    refused(itts, "pairs of columns", ops.q4_matmul, torch.zeros(3, 128, dtype=torch.int8), torch.zeros(3, 2), weight(ops, 17, 100), swiglu=True)
+    x = torch.zeros(3, 130)
+    refused(itts, "on the GPU", ops.q4_linear, x, w)
+    refused(itts, "rows of 130", ops.q4_linear, x[:, :129], w)
+    refused(itts, "norm_weight", ops.q4_linear, x, w, norm_weight=torch.zeros(129))
+    refused(itts, "norm_weight", ops.q4_linear, x, w, norm_weight=torch.zeros(130, dtype=BF16))
+
+
+def test_the_c_abi_refuses(itts, ops):
+    """Addresses that are never read: every call here ends in its checks, with a message."""
+    lib, at = itts._lib, C.c_void_p(1 << 20)
+
+    def norm(x=at, xs=64, res=None, rs=0, w=at, wt=0, t=0, rows=2, cols=64, eps=1e-6, g=64, h=None, hs=0, v=None, vs=0, q=at, s=at):
+        return lib.itts_rmsnorm_q8(x, xs, res, rs, w, wt, t, rows, cols, eps, g, h, hs, v, vs, q, s, None)
+
+    assert norm(rows=0) == 0
+    for kw in ({"x": None}, {"w": None}, {"q": None}, {"s": None}, {"xs": -1}, {"t": 3}, {"t": -1}, {"wt": 1}, {"t": 1, "wt": 2}, {"rows": -1},
+               {"rows": 1 << 40}, {"cols": 0}, {"cols": 1 << 40}, {"eps": -1.0}, {"eps": float("nan")}, {"g": 0}, {"g": 16}, {"h": at, "hs": 63},
+               {"v": at, "vs": 63}, {"res": at, "rs": -1}, {"q": C.c_void_p((1 << 20) + 8)}, {"x": C.c_void_p((1 << 20) + 1)},
+               {"s": C.c_void_p((1 << 20) + 2)}, {"w": C.c_void_p((1 << 20) + 2)}):
+        assert norm(**kw) == -1 and lib.itts_ops_last_error(), kw
+
+    def matmul(q=at, qs=at, rows=2, p=at, s=at, n=32, k=128, g=128, bias=None, res=None, rs=0, flags=0, t=0, out=at, os=32):
+        return lib.itts_q4_matmul(q, qs, rows, p, s, n, k, g, bias, res, rs, flags, t, out, os, None)
+
+    assert matmul(rows=0) == 0
+    for kw in ({"q": None}, {"qs": None}, {"p": None}, {"s": None}, {"out": None}, {"n": 0}, {"n": 1 << 40}, {"k": 0}, {"k": 1 << 40}, {"g": 1},
+               {"flags": 2}, {"t": 7}, {"os": 31}, {"n": 33, "flags": 1, "os": 40}, {"rows": -1}, {"rows": 1 << 40}, {"res": at, "rs": -2},
+               {"q": C.c_void_p((1 << 20) + 4)}, {"p": C.c_void_p((1 << 20) + 4)}, {"out": C.c_void_p((1 << 20) + 2)}, {"bias": C.c_void_p((1 << 20) + 1)}):
+        assert matmul(**kw) == -1, kw
+
+    def linear(x=at, xs=128, xt=0, rows=200, nw=None, wt=0, eps=0.0, p=at, s=at, n=32, k=128, g=128, flags=0, t=0, out=at, os=32, work=at, bytes_=1 << 30):
+        return lib.itts_q4_linear(x, xs, xt, rows, nw, wt, eps, p, s, n, k, g, None, None, 0, flags, t, out, os, work, bytes_, None)
+
+    need = lib.itts_q4_linear_workspace(200, 32, 128, 128)
+    assert need >= 200 * 132 and linear(rows=0) == 0
+    for kw in ({"x": None}, {"xs": -1}, {"xt": 5}, {"nw": at, "wt": 1}, {"nw": at, "eps": -1.0}, {"work": None}, {"bytes_": need - 1},
+               {"work": C.c_void_p((1 << 20) + 16)}, {"out": None}, {"x": C.c_void_p((1 << 20) + 2)}):
+        assert linear(**kw) == -1, kw
+
+    def pack(w=at, ws=128, t=0, n=32, k=128, g=128, p=at, s=at):
+        return lib.itts_q4_pack(w, ws, t, n, k, g, p, s, None)
+
+    def unpack(p=at, s=at, n=32, k=128, g=128, t=0, out=at, os=128):
+        return lib.itts_q4_unpack(p, s, n, k, g, t, out, os, None)
+
+    for kw in ({"w": None}, {"ws": -1}, {"t": 9}, {"n": 0}, {"k": 0}, {"g": 2}, {"p": None}, {"s": None}, {"p": C.c_void_p((1 << 20) + 1)}):
+        assert pack(**kw) == -1, kw
+    for kw in ({"out": None}, {"os": 127}, {"t": 9}, {"n": 0}, {"k": 0}, {"g": 2}, {"p": None}, {"s": None}):
+        assert unpack(**kw) == -1, kw
+    assert lib.itts_q4_packed_bytes(17, 129) == 4 * 1024 and lib.itts_q4_packed_bytes(0, 5) == 0 and lib.itts_q4_packed_bytes(1 << 40, 5) == 0
+    assert lib.itts_q4_scale_count(17, 129, 32) == 4 * 64 and lib.itts_q4_scale_count(17, 129, 31) == 0
