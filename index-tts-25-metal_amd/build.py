@@ -1,6 +1,6 @@
 """Build recipe for libitts_gpt.so (the HIP path + C ABI) and the C++17 drop-in shim.
 
-    python index-tts-25-metal_amd/build.py            # library + shim example
+    python index-tts-25-metal_amd/build.py            # library, torch binding, shim example
     python index-tts-25-metal_amd/build.py --lib-only
 
 Every .hip file is compiled for gfx950 with hipcc, in parallel, into _build/, then
@@ -25,6 +25,7 @@ BUILD = PKG / "_build"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libitts_gpt.so"
 SHIM_EXE = PKG / "cpp" / "gpt_shim_example"
+OPS_MODULE = PKG / "_itts_ops.so"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 DEVICE_FLAGS = [
@@ -81,6 +82,28 @@ def build_library(jobs: int = 8) -> Path:
     return LIB
 
 
+def build_ops_module() -> Path:
+    """The operators' torch binding (host C++ against this interpreter's torch and the C ABI)."""
+    import sysconfig
+
+    import torch
+
+    base = Path(torch.__file__).parent
+    tmp = OPS_MODULE.with_suffix(".tmp")
+    _run([
+        "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        f"-I{INCLUDE}", f"-isystem{base / 'include'}", f"-isystem{base / 'include/torch/csrc/api/include'}",
+        f"-isystem{Path(HIPCC).parent.parent / 'include'}", f"-isystem{sysconfig.get_paths()['include']}",
+        str(CSRC / "ops_torch.cpp"),
+        f"-L{PKG}", "-litts_gpt", f"-L{base / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
+        "-Wl,-rpath,$ORIGIN",
+        "-o", str(tmp),
+    ])
+    os.replace(tmp, OPS_MODULE)
+    return OPS_MODULE
+
+
 def build_shim() -> Path:
     """Compile the C++17 GptDecoder shim and its example against the C ABI (host g++)."""
     cpp = PKG / "cpp"
@@ -105,6 +128,8 @@ def main() -> int:
         print(f"hipcc not found at {HIPCC}", file=sys.stderr)
         return 1
     print(build_library(args.j))
+    if not args.lib_only:
+        print(build_ops_module())
     if not args.lib_only and (PKG / "cpp" / "gpt.cpp").exists():
         print(build_shim())
     return 0

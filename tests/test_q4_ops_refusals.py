@@ -1,6 +1,9 @@
 """What the operators on 4-bit weights and 8-bit activations refuse: checked before anything is enqueued, so
 without a GPU, through itts_ops and through the C ABI."""
 import ctypes as C
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -85,9 +88,40 @@ def test_products(itts, ops):
     refused(itts, "norm_weight", ops.q4_linear, x, w, norm_weight=torch.zeros(130, dtype=BF16))
 
 
+def library(itts):
+    """The C ABI with the argument types of include/itts_ops.h."""
+    lib = C.CDLL(str(itts.LIB_PATH))
+    p, i64, i32, u32, f32, z = C.c_void_p, C.c_int64, C.c_int32, C.c_uint32, C.c_float, C.c_size_t
+    for name, res, args in (
+        ("itts_ops_last_error", C.c_char_p, []),
+        ("itts_rmsnorm_q8", i32, [p, i64, p, i64, p, i32, i32, i64, i64, f32, i32, p, i64, p, i64, p, p, p]),
+        ("itts_q4_packed_bytes", z, [i64, i64]),
+        ("itts_q4_scale_count", z, [i64, i64, i32]),
+        ("itts_q4_pack", i32, [p, i64, i32, i64, i64, i32, p, p, p]),
+        ("itts_q4_unpack", i32, [p, p, i64, i64, i32, i32, p, i64, p]),
+        ("itts_q4_matmul", i32, [p, p, i64, p, p, i64, i64, i32, p, p, i64, u32, i32, p, i64, p]),
+        ("itts_q4_linear_workspace", z, [i64, i64, i64, i32]),
+        ("itts_q4_linear", i32, [p, i64, i32, i64, p, i32, f32, p, p, i64, i64, i32, p, p, i64, u32, i32, p, i64, p, z, p]),
+    ):
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = res, args
+    return lib
+
+
+def test_two_hip_runtimes_are_refused():
+    """torch's streams belong to the HIP runtime that torch brings: with itts_gpt imported first, on the
+    system's runtime, the operators' import says so; the other order works."""
+    pkg = str(Path(__file__).resolve().parent.parent / "index-tts-25-metal_amd")
+    for order, fine in (("import torch, itts_gpt, itts_ops", True), ("import itts_ops", True), ("import itts_gpt, itts_ops", False)):
+        p = subprocess.run([sys.executable, "-c", order], cwd=pkg, capture_output=True, text=True)
+        one = "two HIP runtimes" not in p.stderr
+        # (where torch brings no runtime of its own, there is one in any order)
+        assert (p.returncode == 0) == one and (one or not fine), (order, p.stderr[-500:])
+
+
 def test_the_c_abi_refuses(itts, ops):
     """Addresses that are never read: every call here ends in its checks, with a message."""
-    lib, at = itts._lib, C.c_void_p(1 << 20)
+    lib, at = library(itts), C.c_void_p(1 << 20)
 
     def norm(x=at, xs=64, res=None, rs=0, w=at, wt=0, t=0, rows=2, cols=64, eps=1e-6, g=64, h=None, hs=0, v=None, vs=0, q=at, s=at):
         return lib.itts_rmsnorm_q8(x, xs, res, rs, w, wt, t, rows, cols, eps, g, h, hs, v, vs, q, s, None)
