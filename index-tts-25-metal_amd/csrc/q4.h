@@ -39,6 +39,7 @@ struct ProductArgs {
     int dtype;
     void* out;
     int64_t out_stride;
+    bool wide;             // set by launch_product: rows of out and residual are 16-byte aligned
 };
 hipError_t launch_product(const ProductArgs& a, hipStream_t s);
 

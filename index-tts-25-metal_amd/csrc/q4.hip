@@ -180,50 +180,460 @@ __global__ __launch_bounds__(256) void unpack_kernel(UnpackArgs a) {
 }
 
 // ------------------------------------------------------------------ products
-// One wave per 16 tokens x 16 weight rows, over all columns.
-template <class T, int G, bool SWIGLU>
-__global__ __launch_bounds__(256) void matmul_kernel(ProductArgs a) {
+__device__ __forceinline__ float load_as(const void* p, int64_t i, int dtype) {
+    if (dtype == ITTS_T_F32) return static_cast<const float*>(p)[i];
+    if (dtype == ITTS_T_BF16) return to_float(static_cast<const __bf16*>(p)[i]);
+    return to_float(static_cast<const _Float16*>(p)[i]);
+}
+__device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v) {
+    if (dtype == ITTS_T_F32) static_cast<float*>(p)[i] = v;
+    else if (dtype == ITTS_T_BF16) static_cast<__bf16*>(p)[i] = from_float<__bf16>(v);
+    else static_cast<_Float16*>(p)[i] = from_float<_Float16>(v);
+}
+// What a product adds to the sum of token m and weight row n, read ahead of it.
+struct Added {
+    float bias, residual;
+};
+__device__ __forceinline__ Added added(const ProductArgs& a, int m, int n) {
+    Added e{0.0f, 0.0f};
+    if (m < a.rows && n < a.n) {
+        if (a.bias) e.bias = a.bias[n];
+        if (a.residual) e.residual = load_as(a.residual, m * a.residual_stride + (a.swiglu ? n >> 1 : n), a.dtype);
+    }
+    return e;
+}
+// The last steps of a product's sum.  Lanes next to each other hold weight rows next to each other; all
+// lanes of the wave take part.
+__device__ __forceinline__ void finish(const ProductArgs& a, int m, int n, float v, const Added& e) {
+    v += e.bias;
+    int col = n;
+    bool live = m < a.rows && n < a.n;
+    if (a.swiglu) {
+        v = silu_mul(v, itts::lane_x1(v));
+        col = n >> 1;
+        live = live && !(n & 1);
+    }
+    if (a.residual) v += e.residual;
+    if (live) store_as(a.out, m * a.out_stride + col, a.dtype, v);
+}
+
+// The same for eight weight rows from n, a multiple of eight, at once.
+template <class T, int N>
+__device__ __forceinline__ void finish_row(const ProductArgs& a, int m, int col, int cols, float (&v)[N]) {
+    T* out = static_cast<T*>(a.out) + m * a.out_stride + col;
+    const T* res = a.residual ? static_cast<const T*>(a.residual) + m * a.residual_stride + col : nullptr;
+    struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Piece {
+        T v[N * sizeof(T) < 16 ? N : 16 / sizeof(T)];
+    };
+    constexpr int P = sizeof(Piece) / sizeof(T);
+    if (a.wide && col + N <= cols) {
+#pragma unroll
+        for (int k = 0; k < N / P; ++k) {
+            Piece o;
+            if (res) {
+                const Piece r = reinterpret_cast<const Piece*>(res)[k];
+#pragma unroll
+                for (int i = 0; i < P; ++i) v[k * P + i] += to_float(r.v[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < P; ++i) o.v[i] = from_float<T>(v[k * P + i]);
+            reinterpret_cast<Piece*>(out)[k] = o;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (col + i < cols) out[i] = from_float<T>(res ? v[i] + to_float(res[i]) : v[i]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void finish_typed(const ProductArgs& a, int m, int col, int cols, float (&v)[N]) {
+    if (a.dtype == ITTS_T_F32) finish_row<float, N>(a, m, col, cols, v);
+    else if (a.dtype == ITTS_T_BF16) finish_row<__bf16, N>(a, m, col, cols, v);
+    else finish_row<_Float16, N>(a, m, col, cols, v);
+}
+__device__ __forceinline__ void finish8(const ProductArgs& a, int m, int n, float (&v)[kElems]) {
+    if (m >= a.rows || n >= a.n) return;
+    if (a.bias) {
+#pragma unroll
+        for (int i = 0; i < kElems; ++i) v[i] += a.bias[min(n + i, a.n - 1)];
+    }
+    if (a.swiglu) {
+        float u[kElems / 2];
+#pragma unroll
+        for (int i = 0; i < kElems / 2; ++i) u[i] = silu_mul(v[2 * i], v[2 * i + 1]);
+        finish_typed(a, m, n >> 1, a.n >> 1, u);
+    } else {
+        finish_typed(a, m, n, a.n, v);
+    }
+}
+
+// A few tokens: bound by the weights' bytes and, for small matrices, by latency.  A workgroup owns NT
+// tile rows (16 weight rows each) and all columns; its waves take every W-th tile of 128 columns, U at a
+// time, with all loads of a turn requested before their first use, and add their sums through LDS in
+// wave order.  W hangs on k alone, so a token's result does not depend on the other tokens.
+// The instruction's 16 token rows hold token 16 t + 4 (i % 4) + i / 4 in row i: lane l then ends with
+// tokens 16 t + 4 r + l / 16 in its registers r, and up to 4 (8) tokens take one (two) of the four
+// registers' scaling, which is most of the vector work.
+constexpr int kFewWaves = 8;
+struct FewArgs {
+    ProductArgs p;
+};
+template <int G, int MT, int R, int NT, int U>
+__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
+    extern __shared__ float red[];  // [W][NT * MT * R][64]
+    const ProductArgs& a = fa.p;
+    constexpr int NG = 128 / G, S = NT * MT * R;
     const int lane = threadIdx.x & 63, c = lane & 15, quarter = lane >> 4;
-    const int nt = blockIdx.x * 4 + (threadIdx.x >> 6), m0 = blockIdx.y * 16;
-    const int kb = (a.k + kTileCols - 1) / kTileCols;
-    if (nt * kTileRows >= a.n) return;
-    constexpr int NG = 128 / G;
-    const int8_t* x = a.q + static_cast<int64_t>(min(m0 + c, a.rows - 1)) * kb * kTileCols;
-    const uint8_t* w = a.packed + static_cast<int64_t>(nt) * kb * kTileBytes + lane * 16;
-    const uint16_t* ws = a.wscales + (static_cast<int64_t>(nt) * kb * kTileRows + c) * NG;
-    const float* xs[4];
+    const int W = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kb = (a.k + kTileCols - 1) / kTileCols, nt0 = blockIdx.x * NT, tiles = (a.n + kTileRows - 1) / kTileRows;
+
+    const int8_t* x[MT];
+    const float* xs[MT][R];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) xs[r] = a.qscales + static_cast<int64_t>(min(m0 + 4 * quarter + r, a.rows - 1)) * kb * NG;
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int b = 0; b < kb; ++b) {
-        const TokenCodes xc = token_codes(x + b * kTileCols, lane);
-        const u32x4 wc = *reinterpret_cast<const u32x4*>(w + static_cast<int64_t>(b) * kTileBytes);
-        i32x4 f[NG];
-        tile_product<G>(xc, wc, f);
+    for (int t = 0; t < MT; ++t) {
+        x[t] = a.q + static_cast<int64_t>(min(16 * t + 4 * (c & 3) + (c >> 2), a.rows - 1)) * kb * kTileCols;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const float s = weight_scale(ws[static_cast<int64_t>(b) * kTileRows * NG + g]);
+        for (int r = 0; r < R; ++r) xs[t][r] = a.qscales + static_cast<int64_t>(min(16 * t + 4 * r + quarter, a.rows - 1)) * kb * NG;
+    }
+    const uint8_t* w[NT];
+    const uint16_t* ws[NT];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(static_cast<float>(f[g][r]), xs[r][b * NG + g] * s, acc[r]);
+    for (int i = 0; i < NT; ++i) {
+        const int64_t row = static_cast<int64_t>(min(nt0 + i, tiles - 1)) * kb;
+        w[i] = a.packed + row * kTileBytes + lane * 16;
+        ws[i] = a.wscales + (row * kTileRows + c) * NG;
+    }
+    float acc[NT][MT][R] = {};
+    for (int b0 = wave; b0 < kb; b0 += W * U) {
+        u32x4 wc[U][NT];
+        uint16_t sc[U][NT][NG];
+        TokenCodes xc[U][MT];
+        float xsc[U][MT][R][NG];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int b = min(b0 + u * W, kb - 1);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                wc[u][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(w[i] + static_cast<int64_t>(b) * kTileBytes));
+#pragma unroll
+                for (int g = 0; g < NG; ++g) sc[u][i][g] = ws[i][static_cast<int64_t>(b) * kTileRows * NG + g];
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                xc[u][t] = token_codes(x[t] + b * kTileCols, lane);
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) xsc[u][t][r][g] = xs[t][r][b * NG + g];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (b0 + u * W >= kb) break;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    i32x4 f[NG];
+                    tile_product<G>(xc[u][t], wc[u][i], f);
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        const float s = weight_scale(sc[u][i][g]);
+#pragma unroll
+                        for (int r = 0; r < R; ++r) acc[i][t][r] = __builtin_fmaf(static_cast<float>(f[g][r]), xsc[u][t][r][g] * s, acc[i][t][r]);
+                    }
+                }
         }
     }
-    const int n = nt * kTileRows + c;
-    const float bias = a.bias && n < a.n ? a.bias[n] : 0.0f;
+    auto token = [&](int slot) { return 16 * (slot / R % MT) + 4 * (slot % R) + quarter; };
+    auto row = [&](int slot) { return (nt0 + slot / (MT * R)) * kTileRows + c; };
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int m = m0 + 4 * quarter + r;
-        float v = acc[r] + bias;
-        int col = n;
-        bool live = m < a.rows && n < a.n;
-        if constexpr (SWIGLU) {
-            const float u = itts::lane_x1(v);
-            v = silu_mul(v, u);
-            col = n >> 1;
-            live = live && !(n & 1);
+    for (int s = 0; s < S; ++s) red[(wave * S + s) * 64 + lane] = acc[s / (MT * R)][s / R % MT][s % R];
+    __syncthreads();
+    for (int s = wave; s < S; s += W) {
+        const Added e = added(a, token(s), row(s));
+        float v = 0.0f;
+        for (int k = 0; k < W; ++k) v += red[(k * S + s) * 64 + lane];
+        finish(a, token(s), row(s), v, e);
+    }
+}
+
+// Orders a wave's LDS accesses before and after it.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// 5 to 16 tokens: as few_kernel, with the same sums.  A wave's codes of a tile of columns (16 rows of 128
+// bytes) and their scales go through LDS of its own, whole cache lines at a time: as operands straight from
+// memory, 8 bytes a lane from 16 rows, they took longer than the weights (18.7 -> 8.7 us for 16 x 10240 x 5120).
+constexpr int kCodeRow16 = kTileCols + 8;  // 16 rows' pieces of 8 bytes lie in 32 different banks
+template <int G, int NT>
+__global__ __launch_bounds__(64 * kFewWaves) void batch_kernel(ProductArgs a) {
+    constexpr int NG = 128 / G, kStage = 16 * kCodeRow16 + NG * 16 * 4, S = NT * 4;
+    constexpr int kSums = kFewWaves * S * 256, kCodes = kFewWaves * kStage;
+    __shared__ __align__(16) uint8_t lds[kSums > kCodes ? kSums : kCodes];
+    const int lane = threadIdx.x & 63, c = lane & 15, quarter = lane >> 4;
+    const int W = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kb = (a.k + kTileCols - 1) / kTileCols, nt0 = blockIdx.x * NT, tiles = (a.n + kTileRows - 1) / kTileRows;
+    uint8_t* mine = lds + wave * kStage;
+    float* sums = reinterpret_cast<float*>(lds);
+
+    const int8_t* xg[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) xg[i] = a.q + static_cast<int64_t>(min(8 * i + (lane >> 3), a.rows - 1)) * kb * kTileCols + 16 * (lane & 7);
+    const int token_g = lane / NG, g_of = lane % NG;  // lanes under 16 NG fetch a scale each
+    const float* sg = a.qscales + static_cast<int64_t>(min(min(token_g, 15), a.rows - 1)) * kb * NG + g_of;
+    const uint8_t* w[NT];
+    const uint16_t* ws[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int64_t row = static_cast<int64_t>(min(nt0 + i, tiles - 1)) * kb;
+        w[i] = a.packed + row * kTileBytes + lane * 16;
+        ws[i] = a.wscales + (row * kTileRows + c) * NG;
+    }
+    u32x4 xr[2], wr[NT];
+    float sr = 0.0f;
+    uint16_t wsr[NT][NG];
+    auto fetch = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) xr[i] = *reinterpret_cast<const u32x4*>(xg[i] + b * kTileCols);
+        sr = sg[b * NG];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            wr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(w[i] + static_cast<int64_t>(b) * kTileBytes));
+#pragma unroll
+            for (int g = 0; g < NG; ++g) wsr[i][g] = ws[i][static_cast<int64_t>(b) * kTileRows * NG + g];
         }
-        if (live) {
-            if (a.residual) v += to_float(static_cast<const T*>(a.residual)[m * a.residual_stride + col]);
-            static_cast<T*>(a.out)[m * a.out_stride + col] = from_float<T>(v);
+    };
+    float acc[NT][4] = {};
+    if (wave < kb) fetch(wave);
+    for (int b = wave; b < kb; b += W) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint8_t* at = mine + (8 * i + (lane >> 3)) * kCodeRow16 + 16 * (lane & 7);
+            *reinterpret_cast<uint2*>(at) = make_uint2(xr[i][0], xr[i][1]);
+            *reinterpret_cast<uint2*>(at + 8) = make_uint2(xr[i][2], xr[i][3]);
+        }
+        if (lane < 16 * NG) *reinterpret_cast<float*>(mine + 16 * kCodeRow16 + (g_of * 16 + token_g) * 4) = sr;
+        u32x4 wc[NT];
+        float sc[NT][NG];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            wc[i] = wr[i];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) sc[i][g] = weight_scale(wsr[i][g]);
+        }
+        wave_sync();
+        const TokenCodes xc = token_codes(reinterpret_cast<const int8_t*>(mine) + c * kCodeRow16, lane);
+        float xs[NG][4];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const float4 v = *reinterpret_cast<const float4*>(mine + 16 * kCodeRow16 + (g * 16 + 4 * quarter) * 4);
+            xs[g][0] = v.x, xs[g][1] = v.y, xs[g][2] = v.z, xs[g][3] = v.w;
+        }
+        wave_sync();
+        if (b + W < kb) fetch(b + W);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            i32x4 f[NG];
+            tile_product<G>(xc, wc[i], f);
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][r] = __builtin_fmaf(static_cast<float>(f[g][r]), xs[g][r] * sc[i][g], acc[i][r]);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < S; ++s) sums[(wave * S + s) * 64 + lane] = acc[s / 4][s % 4];
+    __syncthreads();
+    for (int s = wave; s < S; s += W) {
+        const int m = 4 * quarter + s % 4, n = (nt0 + s / 4) * kTileRows + c;
+        const Added e = added(a, m, n);
+        float v = 0.0f;
+        for (int k = 0; k < W; ++k) v += sums[(k * S + s) * 64 + lane];
+        finish(a, m, n, v, e);
+    }
+}
+
+// More than 16 tokens: bound by the scaling.  Every group's 32-bit sums take a conversion, the product of
+// the two scales and a multiply-add a value in the vector units, which at groups of 128 is about what the matrix units need for the
+// group.  A workgroup owns 32 WM MT tokens x 32 WN NT weight rows.  WM x WN waves share a tile of codes staged through
+// LDS; weights go from memory to registers, in the order of the instruction's operand; the next turn's loads
+// are under way while this one's are multiplied.  WK such groups of waves take every WK-th tile of columns and
+// add their sums through LDS in order.
+// v_mfma_i32_32x32x32_i8, not 16x16x64: the same operands give twice the products, and four waves
+// of a SIMD ran them at 35 cycles each against 29 for half the work.
+// The instruction takes 16 consecutive columns from each half of the wave: 64 p + 32 b + 16 h + 0..15 for
+// lane half h, which in a packed tile are the low (b = 0) or high halves of the bytes at 8 p of the lanes of j = 2 h
+// and 2 h + 1.  It leaves weight row l % 32 and tokens 8 (r / 4) + 4 (l / 32) + r % 4 in lane l's registers r.
+typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
+constexpr int kCodeRow = kTileCols + 16;  // eight rows' pieces of 16 bytes lie in 32 different banks
+template <int G, int WM, int WN, int WK, int MT, int NT>
+struct TilesLds {
+    static constexpr int kTokens = WM * MT * 32, kStage = kTokens * (kCodeRow + 128 / G * 4);
+    static constexpr int kSums = WK > 1 ? WK * WM * WN * MT * NT * 4096 : WM * WN * 32 * (NT * 32 + 4) * 4;
+    static constexpr int kBytes = 2 * WK * kStage > kSums ? 2 * WK * kStage : kSums;
+};
+template <int G, int WM, int WN, int WK, int MT, int NT>
+__global__ __launch_bounds__(64 * WM * WN * WK) void tiles_kernel(ProductArgs a) {
+    using Lds = TilesLds<G, WM, WN, WK, MT, NT>;
+    __shared__ __align__(16) uint8_t lds[Lds::kBytes];
+    constexpr int NG = 128 / G, BM = Lds::kTokens, BN = WN * NT * 32, TG = 64 * WM * WN;
+    constexpr int CH = BM * 8 / TG, SC = (BM * NG + TG - 1) / TG;
+    static_assert(BM * 8 % TG == 0, "whole pieces of 16 codes a thread");
+    const int lane = threadIdx.x & 63, c = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wk = wave / (WM * WN), wmn = wave % (WM * WN), wm = wmn / WN, wn = wmn % WN, tg = threadIdx.x - wk * TG;
+    const int kb = (a.k + kTileCols - 1) / kTileCols, tiles = (a.n + kTileRows - 1) / kTileRows;
+    const int mblocks = (a.rows + BM - 1) / BM;
+    const int m0 = blockIdx.x % mblocks * BM, n0 = blockIdx.x / mblocks * BN;
+
+    const int8_t* xg[CH];
+    int xl[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int p = i * TG + tg, r = p >> 3, q = p & 7;
+        xg[i] = a.q + static_cast<int64_t>(min(m0 + r, a.rows - 1)) * kb * kTileCols + 16 * q;
+        xl[i] = r * kCodeRow + 16 * q;
+    }
+    const float* sg[SC];
+    int sl[SC];
+#pragma unroll
+    for (int i = 0; i < SC; ++i) {
+        const int p = min(i * TG + tg, BM * NG - 1), r = p / NG, g = p % NG;
+        sg[i] = a.qscales + static_cast<int64_t>(min(m0 + r, a.rows - 1)) * kb * NG + g;
+        sl[i] = BM * kCodeRow + (g * BM + r) * 4;
+    }
+    const uint8_t* w[NT];
+    const uint16_t* ws[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int64_t row = static_cast<int64_t>(min(n0 / 16 + (wn * NT + i) * 2 + (c >> 4), tiles - 1)) * kb;
+        w[i] = a.packed + row * kTileBytes + (32 * half + (c & 15)) * 16;
+        ws[i] = a.wscales + (row * kTileRows + (c & 15)) * NG;
+    }
+    u32x4 xr[CH], wr[NT][2];
+    float sr[SC];
+    uint16_t wsr[NT][NG];
+    auto fetch = [&](int step) {
+        const int b = min(step * WK + wk, kb - 1);
+#pragma unroll
+        for (int i = 0; i < CH; ++i) xr[i] = *reinterpret_cast<const u32x4*>(xg[i] + b * kTileCols);
+#pragma unroll
+        for (int i = 0; i < SC; ++i) sr[i] = sg[i][b * NG];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const uint8_t* at = w[i] + static_cast<int64_t>(b) * kTileBytes;
+            wr[i][0] = *reinterpret_cast<const u32x4*>(at);
+            wr[i][1] = *reinterpret_cast<const u32x4*>(at + 256);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) wsr[i][g] = ws[i][static_cast<int64_t>(b) * kTileRows * NG + g];
+        }
+    };
+    auto stage = [&](int step) {
+        uint8_t* at = lds + (2 * wk + (step & 1)) * Lds::kStage;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) *reinterpret_cast<u32x4*>(at + xl[i]) = xr[i];
+#pragma unroll
+        for (int i = 0; i < SC; ++i) *reinterpret_cast<float*>(at + sl[i]) = sr[i];
+    };
+    float acc[NT][MT][16] = {};
+    const int steps = (kb + WK - 1) / WK;
+    fetch(0);
+    stage(0);
+    for (int step = 0; step < steps; ++step) {
+        u32x4 wc[NT][2];
+        float sc[NT][NG];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            wc[i][0] = wr[i][0];
+            wc[i][1] = wr[i][1];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) sc[i][g] = weight_scale(wsr[i][g]);
+        }
+        __syncthreads();
+        if (step + 1 < steps) fetch(step + 1);
+        if (step * WK + wk < kb) {
+            const uint8_t* at = lds + (2 * wk + (step & 1)) * Lds::kStage;
+            i32x4 xc[MT][4];
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) xc[t][q] = *reinterpret_cast<const i32x4*>(at + ((wm * MT + t) * 32 + c) * kCodeRow + 32 * q + 16 * half);
+            const uint8_t* xs = at + BM * kCodeRow + (wm * MT * 32 + 4 * half) * 4;
+            // the products of one block of 32 x 32 and group are under way while those of the one before are scaled
+            i32x16 f[2];
+            auto multiply = [&](int i, int t, int g, i32x16& to) {
+                const i32x16 zero = {};
+                constexpr int Q = G / 32;
+#pragma unroll
+                for (int q = g * Q; q < (g + 1) * Q; ++q) {
+                    const int p = q >> 1;
+                    i32x4 wq;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t v = wc[i][e >> 1][2 * p + (e & 1)];
+                        wq[e] = static_cast<int>((q & 1 ? v : v << 4) & kHigh);
+                    }
+                    to = __builtin_amdgcn_mfma_i32_32x32x32_i8(xc[t][q], wq, q == g * Q ? zero : to, 0, 0, 0);
+                }
+            };
+            auto scale = [&](int i, int t, int g, const i32x16& from) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float4 v = *reinterpret_cast<const float4*>(xs + (g * BM + t * 32 + 8 * q) * 4);
+                    const float x4[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        acc[i][t][4 * q + r] = __builtin_fmaf(static_cast<float>(from[4 * q + r]), x4[r] * sc[i][g], acc[i][t][4 * q + r]);
+                }
+            };
+#pragma unroll
+            for (int j = 0; j < NT * MT * NG; ++j) {
+                multiply(j / (MT * NG), j / NG % MT, j % NG, f[j & 1]);
+                if (j > 0) scale((j - 1) / (MT * NG), (j - 1) / NG % MT, (j - 1) % NG, f[(j - 1) & 1]);
+            }
+            scale(NT - 1, MT - 1, NG - 1, f[(NT * MT * NG - 1) & 1]);
+        }
+        if (step + 1 < steps) stage(step + 1);
+    }
+    __syncthreads();
+    if constexpr (WK == 1) {
+        // thirty-two tokens at a time through LDS, so that a lane has eight columns of one token
+        constexpr int BW = NT * 32, LR = BW / 8;  // columns of the wave, lanes a token
+        float* mine = reinterpret_cast<float*>(lds) + wave * (32 * (BW + 4));
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mine[(8 * (r >> 2) + 4 * half + (r & 3)) * (BW + 4) + i * 32 + c] = acc[i][t][r];
+            wave_sync();
+            for (int r0 = 0; r0 < 32; r0 += 64 / LR) {
+                const int r = r0 + lane / LR, col = lane % LR * 8;
+                float v[kElems];
+#pragma unroll
+                for (int e = 0; e < kElems; ++e) v[e] = mine[r * (BW + 4) + col + e];
+                finish8(a, m0 + (wm * MT + t) * 32 + r, n0 + wn * BW + col, v);
+            }
+            wave_sync();
+        }
+    } else {
+        constexpr int S = NT * MT * 16;
+        float* sums = reinterpret_cast<float*>(lds);
+#pragma unroll
+        for (int s = 0; s < S; ++s) sums[(wave * S + s) * 64 + lane] = acc[s / (MT * 16)][s / 16 % MT][s % 16];
+        __syncthreads();
+        for (int j = wave; j < WM * WN * S; j += WM * WN * WK) {
+            const int o = j / S, s = j % S, r = s % 16;
+            const int m = m0 + (o / WN * MT + s / 16 % MT) * 32 + 8 * (r >> 2) + 4 * half + (r & 3), n = n0 + (o % WN * NT + s / (MT * 16)) * 32 + c;
+            const Added e = added(a, m, n);
+            float v = 0.0f;
+#pragma unroll
+            for (int k = 0; k < WK; ++k) v += sums[((k * WM * WN + o) * S + s) * 64 + lane];
+            finish(a, m, n, v, e);
         }
     }
 }
@@ -280,18 +690,70 @@ hipError_t launch_rows(const NormArgs& a, hipStream_t s) {
     });
 }
 
-hipError_t launch_product(const ProductArgs& a, hipStream_t s) {
-    if (a.rows == 0) return hipSuccess;
-    const dim3 grid((a.n + 63) / 64, (a.rows + 15) / 16);
-    return by_type(a.dtype, [&](auto t) {
-        using T = decltype(t);
-        return by_group(a.group, [&](auto g) {
-            return by_bool(a.swiglu, [&](auto sw) {
-                hipLaunchKernelGGL((matmul_kernel<T, decltype(g)::value, decltype(sw)::value>), grid, dim3(256), 0, s, a);
-                return hipGetLastError();
-            });
-        });
-    });
+namespace {
+constexpr int kFewWide = 32768;
+
+template <int G, int MT, int R, int NT, int U>
+hipError_t launch_few(const ProductArgs& a, hipStream_t s) {
+    const int kb = pad_cols(a.k) / kTileCols, W = std::min(kb, kFewWaves);
+    const int tiles = (a.n + kTileRows - 1) / kTileRows;
+    hipLaunchKernelGGL((few_kernel<G, MT, R, NT, U>), dim3((tiles + NT - 1) / NT), dim3(64 * W), W * NT * MT * R * 64 * sizeof(float), s, FewArgs{a});
+    return hipGetLastError();
+}
+template <int G, int NT>
+hipError_t launch_batch(const ProductArgs& a, hipStream_t s) {
+    const int kb = pad_cols(a.k) / kTileCols, tiles = (a.n + kTileRows - 1) / kTileRows;
+    hipLaunchKernelGGL((batch_kernel<G, NT>), dim3((tiles + NT - 1) / NT), dim3(64 * std::min(kb, kFewWaves)), 0, s, a);
+    return hipGetLastError();
+}
+template <int G, int WM, int WN, int WK, int MT, int NT>
+hipError_t launch_tiles(const ProductArgs& a, hipStream_t s) {
+    const int mb = (a.rows + WM * MT * 32 - 1) / (WM * MT * 32), nb = (a.n + WN * NT * 32 - 1) / (WN * NT * 32);
+    hipLaunchKernelGGL((tiles_kernel<G, WM, WN, WK, MT, NT>), dim3(static_cast<unsigned>(mb) * nb), dim3(64 * WM * WN * WK), 0, s, a);
+    return hipGetLastError();
+}
+template <int G>
+hipError_t product(const ProductArgs& a, hipStream_t s) {
+    if (a.rows <= 4) {
+        if (a.n >= kFewWide) return launch_few<G, 1, 1, 4, 1>(a, s);
+        return launch_few<G, 1, 1, 1, 4>(a, s);
+    }
+#ifdef VAR
+    const int var = std::getenv("VAR") ? std::atoi(std::getenv("VAR")) : 0;
+    switch (var) {
+        case 1: return launch_batch<G, 1>(a, s);
+        case 2: return launch_batch<G, 2>(a, s);
+        case 3: return launch_batch<G, 4>(a, s);
+        case 4: return launch_tiles<G, 1, 1, 8, 1, 1>(a, s);
+        case 5: return launch_tiles<G, 1, 1, 4, 1, 1>(a, s);
+        case 6: return launch_tiles<G, 1, 2, 4, 1, 1>(a, s);
+        case 7: return launch_tiles<G, 1, 4, 2, 1, 1>(a, s);
+        case 8: return launch_tiles<G, 1, 4, 1, 1, 1>(a, s);
+        case 9: return launch_tiles<G, 2, 1, 4, 1, 1>(a, s);
+        case 10: return launch_tiles<G, 2, 2, 2, 1, 1>(a, s);
+        case 11: return launch_tiles<G, 2, 2, 1, 1, 1>(a, s);
+        case 12: return launch_tiles<G, 1, 4, 1, 2, 1>(a, s);
+        case 13: return launch_tiles<G, 2, 2, 1, 2, 1>(a, s);
+        case 14: return launch_tiles<G, 2, 2, 1, 2, 2>(a, s);
+        case 15: return launch_tiles<G, 2, 4, 1, 2, 1>(a, s);
+        case 16: return launch_tiles<G, 2, 2, 2, 2, 1>(a, s);
+        case 17: return launch_tiles<G, 1, 4, 1, 4, 1>(a, s);
+        case 18: return launch_tiles<G, 4, 2, 1, 1, 1>(a, s);
+        case 19: return launch_tiles<G, 2, 4, 1, 2, 2>(a, s);
+    }
+#endif
+    if (a.rows <= 16) return launch_batch<G, 1>(a, s);
+    if (a.rows <= 32) return launch_tiles<G, 1, 1, 8, 1, 1>(a, s);
+    if (a.rows <= 64) return launch_tiles<G, 2, 1, 4, 1, 1>(a, s);
+    return launch_tiles<G, 2, 2, 1, 2, 1>(a, s);
+}
+}  // namespace
+
+hipError_t launch_product(const ProductArgs& given, hipStream_t s) {
+    if (given.rows == 0) return hipSuccess;
+    ProductArgs a = given;
+    a.wide = rows_aligned(a.out, a.out_stride, a.dtype) && rows_aligned(a.residual, a.residual_stride, a.dtype);
+    return by_group(a.group, [&](auto g) { return product<decltype(g)::value>(a, s); });
 }
 
 hipError_t launch_pack(const void* w, int64_t stride, int dtype, int n, int k, int group, void* packed, void* scales, hipStream_t s) {
