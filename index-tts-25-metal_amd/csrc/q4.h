@@ -43,6 +43,23 @@ struct ProductArgs {
 };
 hipError_t launch_product(const ProductArgs& a, hipStream_t s);
 
+// A product of up to four rows, or (launch_fused) the norm or quantisation of one row and its product, with what a
+// decode step adds to them.
+struct FewArgs {
+    ProductArgs p;           // (launch_fused: without q, qscales)
+    NormArgs rows;           // launch_fused: x, x_stride, weight, weight_dtype, dtype, cols, eps
+    const uint32_t* active;  // or null: the launch does nothing where it is 0
+    const uint32_t* token;   // or null: x is row *token of a matrix (launch_fused)
+    float* h_out;            // or null: receives x's row in F32 (launch_fused)
+    float2* best;            // or null: per 16 weight rows the largest sum of row 0 and its index
+    bool vec;                // set by launch_fused
+};
+hipError_t launch_few(const FewArgs& a, hipStream_t s);
+bool linear_is_fused(int64_t rows, int64_t n, int64_t k);
+hipError_t launch_fused(const FewArgs& a, hipStream_t s);
+// Norm (or quantisation) and product: fused, or through rows.q and rows.scales.
+hipError_t launch_linear(const ProductArgs& p, const NormArgs& rows, hipStream_t s);
+
 hipError_t launch_pack(const void* w, int64_t stride, int dtype, int n, int k, int group, void* packed, void* scales, hipStream_t s);
 hipError_t launch_unpack(const void* packed, const void* scales, int n, int k, int group, int dtype, void* out, int64_t stride, hipStream_t s);
 

@@ -10,70 +10,115 @@
 namespace itts {
 namespace q4 {
 
+// Elements of a type known at run time, as load_row; vec: as its VEC.
+template <int E>
+__device__ __forceinline__ void load_row_as(const void* row, int64_t c, int64_t cols, int dtype, bool vec, float (&out)[E]) {
+    if (dtype == ITTS_T_F32) {
+        if (vec) load_row<true>(static_cast<const float*>(row), c, cols, out);
+        else load_row<false>(static_cast<const float*>(row), c, cols, out);
+    } else if (dtype == ITTS_T_BF16) {
+        if (vec) load_row<true>(static_cast<const __bf16*>(row), c, cols, out);
+        else load_row<false>(static_cast<const __bf16*>(row), c, cols, out);
+    } else {
+        if (vec) load_row<true>(static_cast<const _Float16*>(row), c, cols, out);
+        else load_row<false>(static_cast<const _Float16*>(row), c, cols, out);
+    }
+}
+
 // ------------------------------------------------------------------ rows to 8 bits
-// One workgroup per row: the row's squares in a first pass (which writes h), its codes in a second one
-// that reads h again.
+// Bound by memory: every element is read once.  A team of waves owns a row and keeps it in registers between the
+// two passes, CH runs of eight columns a lane; the norm's weights are requested with the row.  CH = 0: rows
+// longer than that, by 1024 threads, which read h (or x) again.
 struct RowsArgs {
     NormArgs a;
-    int kp;
+    int kp, waves;  // padded columns; waves of a team
 };
+constexpr int kLongThreads = 1024;
 
-template <class T, class WT, int G, bool NORM, bool VEC>
-__global__ __launch_bounds__(256) void rows_kernel(RowsArgs ra) {
+template <class T, int CH, bool VEC>
+__global__ __launch_bounds__(1024) void rows_kernel(RowsArgs ra) {
     const NormArgs& a = ra.a;
-    __shared__ double red[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    constexpr int N = CH ? CH : 1;
+    constexpr int kBlocks = CH ? 16 * 4 * CH : 64;  // blocks of 128 columns: up to 16 waves of 4 CH
+    __shared__ double blocks[kBlocks];
+    const int lane = threadIdx.x & 63, waves = ra.waves, teams = blockDim.x / (64 * waves);
+    const int team = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6) / waves), tid = threadIdx.x - team * waves * 64;
+    const int step = waves * 64 * kElems, kb = ra.kp / kTileCols, passes = CH ? CH : (ra.kp + step - 1) / step;
+    double* mine = blocks + team * (kBlocks / teams);
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * teams; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * teams) {
+        const int64_t r = r0 + team;
+        const bool live = r < a.rows;
         const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
         const T* res = a.residual ? static_cast<const T*>(a.residual) + r * a.residual_stride : nullptr;
         T* h = a.h_out ? static_cast<T*>(a.h_out) + r * a.h_stride : nullptr;
-        auto hidden = [&](int64_t c, float (&v)[kElems]) {
-            load8<VEC>(x, c, a.cols, v);
+        float v[N][kElems], w[N][kElems];
+        // (rows behind the last one count as empty)
+        auto hidden = [&](int64_t c, float (&to)[kElems]) {
+            load_row<VEC>(x, c, live ? a.cols : 0, to);
             if (res) {
                 float u[kElems];
-                load8<VEC>(res, c, a.cols, u);
+                load_row<VEC>(res, c, live ? a.cols : 0, u);
 #pragma unroll
-                for (int i = 0; i < kElems; ++i) v[i] = to_float(from_float<T>(v[i] + u[i]));
+                for (int i = 0; i < kElems; ++i) to[i] = to_float(from_float<T>(to[i] + u[i]));
             }
         };
-        double inv = 1.0;
-        if constexpr (NORM) {
-            double ss = 0.0;
-            for (int64_t c = tid * kElems; c < a.cols; c += 256 * kElems) {
-                float v[kElems];
-                hidden(c, v);
+        if constexpr (CH > 0) {
 #pragma unroll
-                for (int i = 0; i < kElems; ++i) ss = fma(static_cast<double>(v[i]), static_cast<double>(v[i]), ss);
+            for (int i = 0; i < CH; ++i) hidden(tid * kElems + i * step, v[i]);
+            if (a.weight) {
+#pragma unroll
+                for (int i = 0; i < CH; ++i) load_row_as(a.weight, tid * kElems + i * step, a.cols, a.weight_dtype, VEC, w[i]);
             }
-            ss = wave_sum64(ss);
-            if (lane == 0) red[wave] = ss;
-            __syncthreads();
-            ss = (red[0] + red[1]) + (red[2] + red[3]);
-            __syncthreads();
-            inv = 1.0 / sqrt(ss / static_cast<double>(a.cols) + static_cast<double>(a.eps));
         }
-        for (int64_t c = tid * kElems; c < ra.kp; c += 256 * kElems) {
-            float v[kElems];
-            hidden(c, v);
-            if (h) store8<VEC>(h, c, a.cols, v);
-            double z[kElems];
-            if constexpr (NORM) {
-                float w[kElems];
-                load8<VEC>(static_cast<const WT*>(a.weight), c, a.cols, w);
-#pragma unroll
-                for (int i = 0; i < kElems; ++i) z[i] = static_cast<double>(v[i]) * static_cast<double>(w[i]);
+        double inv = 1.0;
+        if (a.weight) {
+            double sum = 0.0;
+            for (int i = 0; i < passes; ++i) {
+                if constexpr (CH == 0) {
+                    hidden(tid * kElems + static_cast<int64_t>(i) * step, v[0]);
+                    sum += block_squares<kElems>(lane_squares(v[0]));  // of block tid / 16 + 64 i
+                }
+            }
+            if constexpr (CH == 0) {
+                if (tid % 16 == 0) mine[tid / 16] = sum;
             } else {
 #pragma unroll
-                for (int i = 0; i < kElems; ++i) z[i] = static_cast<double>(v[i]);
+                for (int i = 0; i < CH; ++i) {
+                    const double s = block_squares<kElems>(lane_squares(v[i]));
+                    const int b = (tid + i * waves * 64) / 16;
+                    if (tid % 16 == 0 && b < kb) mine[b] = s;
+                }
             }
-            int8_t code[kElems];
-            const float s = group_codes<G>(z, inv, c - c % G < a.cols, code);
-            *reinterpret_cast<uint2*>(a.q + r * ra.kp + c) = pack_codes(code);
-            if (c % G == 0) a.scales[r * (ra.kp / G) + c / G] = s;
-            if (a.values) {
+            __syncthreads();
+            inv = inv_rms(row_squares(mine, CH ? kb : 64, lane), a);
+            __syncthreads();
+        }
+        auto codes = [&](int64_t c, float (&hv)[kElems], float (&wv)[kElems]) {
+            if (!live || c >= ra.kp) return;  // (whole groups)
+            if (h) store_row<VEC>(h, c, a.cols, hv);
+            double z[kElems];
 #pragma unroll
-                for (int i = 0; i < kElems; ++i) v[i] = static_cast<float>(code[i]) * s;
-                store8<VEC>(static_cast<T*>(a.values) + r * a.values_stride, c, a.cols, v);
+            for (int i = 0; i < kElems; ++i) z[i] = a.weight ? static_cast<double>(hv[i]) * static_cast<double>(wv[i]) : static_cast<double>(hv[i]);
+            int8_t code[kElems];
+            const float s = group_codes(z, inv, a.group, c - c % a.group < a.cols, code);
+            *reinterpret_cast<uint2*>(a.q + r * ra.kp + c) = make_uint2(four_codes(code), four_codes(code + 4));
+            if (c % a.group == 0) a.scales[r * (ra.kp / a.group) + c / a.group] = s;
+            if (a.values) {
+                float u[kElems];
+#pragma unroll
+                for (int i = 0; i < kElems; ++i) u[i] = static_cast<float>(code[i]) * s;
+                store_row<VEC>(static_cast<T*>(a.values) + r * a.values_stride, c, a.cols, u);
+            }
+        };
+        if constexpr (CH > 0) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) codes(tid * kElems + i * step, v[i], w[i]);
+        } else {
+            for (int i = 0; i < passes; ++i) {
+                const int64_t c = tid * kElems + static_cast<int64_t>(i) * step;
+                hidden(c, v[0]);
+                if (a.weight) load_row_as(a.weight, c, a.cols, a.weight_dtype, VEC, w[0]);
+                codes(c, v[0], w[0]);
             }
         }
     }
@@ -103,7 +148,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     const T* src = static_cast<const T*>(a.w) + row * a.stride;
     float v[4][kElems];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) load8<VEC>(src, c0 + 32 * b, row < a.n ? a.k : 0, v[b]);
+    for (int b = 0; b < 4; ++b) load_row<VEC>(src, c0 + 32 * b, row < a.n ? a.k : 0, v[b]);
     uint32_t out[4] = {0, 0, 0, 0};
     constexpr int B = G / 32, NG = 4 / B;
     uint16_t sc[NG];
@@ -175,7 +220,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(UnpackArgs a) {
             const int shift = 8 * (i & 3) + 4 * (b & 1);
             v[i] = static_cast<float>(static_cast<int32_t>(w[2 * (b >> 1) + (i >> 2)] << (28 - shift)) >> 28) * s;
         }
-        store8<VEC>(dst, c0 + 32 * b, a.k, v);
+        store_row<VEC>(dst, c0 + 32 * b, a.k, v);
     }
 }
 
@@ -267,101 +312,190 @@ __device__ __forceinline__ void finish8(const ProductArgs& a, int m, int n, floa
     }
 }
 
-// A few tokens: bound by the weights' bytes and, for small matrices, by latency.  A workgroup owns NT
-// tile rows (16 weight rows each) and all columns; its waves take every W-th tile of 128 columns, U at a
-// time, with all loads of a turn requested before their first use, and add their sums through LDS in
-// wave order.  W hangs on k alone, so a token's result does not depend on the other tokens.
-// The instruction's 16 token rows hold token 16 t + 4 (i % 4) + i / 4 in row i: lane l then ends with
-// tokens 16 t + 4 r + l / 16 in its registers r, and up to 4 (8) tokens take one (two) of the four
-// registers' scaling, which is most of the vector work.
-constexpr int kFewWaves = 8;
-struct FewArgs {
-    ProductArgs p;
-};
-template <int G, int MT, int R, int NT, int U>
-__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
-    extern __shared__ float red[];  // [W][NT * MT * R][64]
-    const ProductArgs& a = fa.p;
-    constexpr int NG = 128 / G, S = NT * MT * R;
-    const int lane = threadIdx.x & 63, c = lane & 15, quarter = lane >> 4;
-    const int W = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kb = (a.k + kTileCols - 1) / kTileCols, nt0 = blockIdx.x * NT, tiles = (a.n + kTileRows - 1) / kTileRows;
-
-    const int8_t* x[MT];
-    const float* xs[MT][R];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        x[t] = a.q + static_cast<int64_t>(min(16 * t + 4 * (c & 3) + (c >> 2), a.rows - 1)) * kb * kTileCols;
-#pragma unroll
-        for (int r = 0; r < R; ++r) xs[t][r] = a.qscales + static_cast<int64_t>(min(16 * t + 4 * r + quarter, a.rows - 1)) * kb * NG;
-    }
-    const uint8_t* w[NT];
-    const uint16_t* ws[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        const int64_t row = static_cast<int64_t>(min(nt0 + i, tiles - 1)) * kb;
-        w[i] = a.packed + row * kTileBytes + lane * 16;
-        ws[i] = a.wscales + (row * kTileRows + c) * NG;
-    }
-    float acc[NT][MT][R] = {};
-    for (int b0 = wave; b0 < kb; b0 += W * U) {
-        u32x4 wc[U][NT];
-        uint16_t sc[U][NT][NG];
-        TokenCodes xc[U][MT];
-        float xsc[U][MT][R][NG];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int b = min(b0 + u * W, kb - 1);
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                wc[u][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(w[i] + static_cast<int64_t>(b) * kTileBytes));
-#pragma unroll
-                for (int g = 0; g < NG; ++g) sc[u][i][g] = ws[i][static_cast<int64_t>(b) * kTileRows * NG + g];
-            }
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                xc[u][t] = token_codes(x[t] + b * kTileCols, lane);
-#pragma unroll
-                for (int r = 0; r < R; ++r)
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) xsc[u][t][r][g] = xs[t][r][b * NG + g];
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (b0 + u * W >= kb) break;
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    i32x4 f[NG];
-                    tile_product<G>(xc[u][t], wc[u][i], f);
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        const float s = weight_scale(sc[u][i][g]);
-#pragma unroll
-                        for (int r = 0; r < R; ++r) acc[i][t][r] = __builtin_fmaf(static_cast<float>(f[g][r]), xsc[u][t][r][g] * s, acc[i][t][r]);
-                    }
-                }
-        }
-    }
-    auto token = [&](int slot) { return 16 * (slot / R % MT) + 4 * (slot % R) + quarter; };
-    auto row = [&](int slot) { return (nt0 + slot / (MT * R)) * kTileRows + c; };
-#pragma unroll
-    for (int s = 0; s < S; ++s) red[(wave * S + s) * 64 + lane] = acc[s / (MT * R)][s / R % MT][s % R];
-    __syncthreads();
-    for (int s = wave; s < S; s += W) {
-        const Added e = added(a, token(s), row(s));
-        float v = 0.0f;
-        for (int k = 0; k < W; ++k) v += red[(k * S + s) * 64 + lane];
-        finish(a, token(s), row(s), v, e);
-    }
+// The largest of a tile's 16 sums (token 0: lanes 0 to 15), the first of equal ones; of NaN and -inf alone: -inf, row 0.
+__device__ __forceinline__ void tile_best(float2* best, int tile, int tiles, float v, int n, int lane) {
+    float i = __int_as_float(n);
+    if (!(v > -INFINITY)) v = -INFINITY, i = __int_as_float(0);
+    auto take = [&](float ov, float oi) {
+        if (ov > v || (ov == v && __float_as_int(oi) < __float_as_int(i))) v = ov, i = oi;
+    };
+    take(itts::lane_x8(v), itts::lane_x8(i));
+    take(itts::lane_x4(v), itts::lane_x4(i));
+    take(itts::lane_x2(v), itts::lane_x2(i));
+    take(itts::lane_x1(v), itts::lane_x1(i));
+    if (lane == 0 && tile < tiles) best[tile] = make_float2(v, i);
 }
 
 // Orders a wave's LDS accesses before and after it.
 __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+}
+
+// Up to four tokens: bound by the weights' bytes and, for small matrices, by latency.  A workgroup owns NT
+// tile rows (16 weight rows each) and all columns; its waves take every W-th tile of 128 columns, U at a
+// time, with all loads of a turn requested before their first use, and add their sums through LDS in
+// wave order.  W hangs on k alone, so a token's result does not depend on the other tokens.
+// The instruction's token rows 4 i hold token i: lane l then ends with token l / 16 in its first register, and
+// the other three are not scaled, which is most of the vector work.
+// FUSED: one token as a float row.  Every workgroup norms it and forms its codes in LDS, with its first
+// turn's weights already under way: one launch instead of two, 6.4 -> 4.2 us for one row x 4096 x 1024.
+// (Four rows by every workgroup took longer than a launch of their own: 14.8 us against 8.4 for 4 x 10240 x 1280.)
+constexpr int kFewWaves = 8, kFewTokens = 4, kFusedCols = 16384;
+constexpr int kFewRow = kTileCols + 8;  // four rows' pieces lie in different banks
+template <int G, int NT, int U, bool FUSED>
+__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
+    const ProductArgs& a = fa.p;
+    if (fa.active && !*fa.active) return;
+    constexpr int NG = 128 / G;
+    // codes by blocks of 128 columns: [block][token][136 bytes], and scales [block][token][NG]; all blocks
+    // of one token (FUSED), or those of a wave's turn
+    constexpr int kBlocks = FUSED ? kFusedCols / kTileCols : kFewWaves * U * kFewTokens;
+    __shared__ __align__(16) uint8_t codes[kBlocks * kFewRow];
+    __shared__ float scales[kBlocks * NG];
+    __shared__ float sums[kFewWaves * NT * 64];
+    __shared__ double squares[FUSED ? kFusedCols / kTileCols : 1];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, quarter = lane >> 4;
+    const int W = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kb = (a.k + kTileCols - 1) / kTileCols, tiles = (a.n + kTileRows - 1) / kTileRows;
+    const int rows = a.rows, mine = min(c >> 2, rows - 1), scaled = min(quarter, rows - 1);  // (c & 3 > 0: whatever)
+
+    u32x4 wc[U][NT];
+    uint16_t sc[U][NT][NG];
+    auto weights = [&](int run, int b0) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int64_t row = static_cast<int64_t>(min(run * NT + i, tiles - 1)) * kb;
+            const uint8_t* w = a.packed + row * kTileBytes + lane * 16;
+            const uint16_t* ws = a.wscales + (row * kTileRows + c) * NG;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t b = min(b0 + u * W, kb - 1);
+                wc[u][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(w + b * kTileBytes));
+#pragma unroll
+                for (int g = 0; g < NG; ++g) sc[u][i][g] = ws[b * kTileRows * NG + g];
+            }
+        }
+    };
+    if constexpr (FUSED) {
+        weights(blockIdx.x, wave);
+        const NormArgs& r = fa.rows;
+        const int T = blockDim.x, quads = kb * 32;
+        const int64_t first = fa.token ? *fa.token : 0;
+        const uint8_t* row = static_cast<const uint8_t*>(r.x) + first * r.x_stride * (r.dtype == ITTS_T_F32 ? 4 : 2);
+        // four columns a thread, half a wave a block; the first two turns stay in registers between the passes
+        constexpr int KEEP = 2;
+        float v0[KEEP][4], g0[KEEP][4];
+        auto fetch = [&](int p, float (&v)[4], float (&g)[4]) {
+            load_row_as(row, p * 4, a.k, r.dtype, fa.vec, v);
+            if (r.weight) load_row_as(r.weight, p * 4, a.k, r.weight_dtype, fa.vec, g);
+        };
+        auto norm = [&](int p, const float (&v)[4]) {
+            const double s = block_squares<4>(lane_squares(v));
+            if ((p & 31) == 0) squares[p >> 5] = s;
+        };
+        double inv = 1.0;
+        auto quantise = [&](int p, const float (&v)[4], const float (&g)[4]) {
+            const int col = p * 4;
+            if (fa.h_out && blockIdx.x == 0) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col + e < a.k) fa.h_out[col + e] = v[e];
+            }
+            double z[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] = r.weight ? static_cast<double>(v[e]) * static_cast<double>(g[e]) : static_cast<double>(v[e]);
+            int8_t code[4];
+            const float s = group_codes(z, inv, G, col - col % G < a.k, code);
+            *reinterpret_cast<uint32_t*>(codes + (p >> 5) * kFewRow + (p & 31) * 4) = four_codes(code);
+            if (col % G == 0) scales[col / G] = s;
+        };
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i)
+            if (tid + i * T < quads) fetch(tid + i * T, v0[i], g0[i]);
+        if (r.weight) {
+#pragma unroll
+            for (int i = 0; i < KEEP; ++i)
+                if (tid + i * T < quads) norm(tid + i * T, v0[i]);
+            for (int p = tid + KEEP * T; p < quads; p += T) {
+                float v[4], g[4];
+                fetch(p, v, g);
+                norm(p, v);
+            }
+            __syncthreads();
+            if (wave * 64 < quads) inv = inv_rms(row_squares(squares, kb, lane), r);
+        }
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i)
+            if (tid + i * T < quads) quantise(tid + i * T, v0[i], g0[i]);
+        for (int p = tid + KEEP * T; p < quads; p += T) {
+            float v[4], g[4];
+            fetch(p, v, g);
+            quantise(p, v, g);
+        }
+        __syncthreads();
+    }
+    // the wave's own places for a turn's codes and scales, which whole cache lines bring there
+    const int own = wave * U * kFewTokens, piece = lane & 7, token_c = min(lane >> 3, rows - 1);
+    const int8_t* xg = FUSED ? nullptr : a.q + static_cast<int64_t>(token_c) * kb * kTileCols + 16 * piece;
+    const float* sg = FUSED ? nullptr : a.qscales + static_cast<int64_t>(min(lane / NG, rows - 1)) * kb * NG + lane % NG;
+
+    {
+        const int run = blockIdx.x;
+        float acc[NT] = {};
+        for (int b0 = wave; b0 < kb; b0 += W * U) {
+            if (!FUSED || b0 != wave) weights(run, b0);
+            if constexpr (!FUSED) {
+                u32x4 xr[U];
+                float sr[U];
+                if (lane < 8 * kFewTokens) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int b = min(b0 + u * W, kb - 1);
+                        xr[u] = *reinterpret_cast<const u32x4*>(xg + b * kTileCols);
+                        sr[u] = lane < kFewTokens * NG ? sg[b * NG] : 0.0f;
+                    }
+                    wave_sync();
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        uint8_t* at = codes + (own + u * kFewTokens + (lane >> 3)) * kFewRow + 16 * piece;
+                        *reinterpret_cast<uint2*>(at) = make_uint2(xr[u][0], xr[u][1]);
+                        *reinterpret_cast<uint2*>(at + 8) = make_uint2(xr[u][2], xr[u][3]);
+                        if (lane < kFewTokens * NG) scales[(own + u * kFewTokens) * NG + lane] = sr[u];
+                    }
+                }
+                wave_sync();
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int b = b0 + u * W;
+                if (b >= kb) break;
+                const int at = FUSED ? b : own + u * kFewTokens;
+                const TokenCodes xc = token_codes(reinterpret_cast<const int8_t*>(codes) + (at + mine) * kFewRow, lane);
+                float xs[NG];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) xs[g] = scales[(at + scaled) * NG + g];
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    i32x4 f[NG];
+                    tile_product<G>(xc, wc[u][i], f);
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) acc[i] = __builtin_fmaf(static_cast<float>(f[g][0]), xs[g] * weight_scale(sc[u][i][g]), acc[i]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) sums[(wave * NT + i) * 64 + lane] = acc[i];
+        __syncthreads();
+        for (int i = wave; i < NT; i += W) {
+            const int n = (run * NT + i) * kTileRows + c;
+            const Added e = added(a, quarter, n);
+            float v = 0.0f;
+            for (int k = 0; k < W; ++k) v += sums[(k * NT + i) * 64 + lane];
+            finish(a, quarter, n, v, e);
+            if (fa.best) tile_best(fa.best, run * NT + i, tiles, n < a.n ? v : -INFINITY, n, lane);
+        }
+    }
 }
 
 // 5 to 16 tokens: as few_kernel, with the same sums.  A wave's codes of a tile of columns (16 rows of 128
@@ -661,44 +795,68 @@ hipError_t by_bool(bool b, F&& f) {
     return b ? f(Int<1>()) : f(Int<0>());
 }
 size_t type_size(int dtype) { return dtype == ITTS_T_F32 ? 4 : 2; }
-// Rows that load8 and store8 may take 16 bytes at a time.
+// Rows that load_row and store_row may take 16 bytes at a time.
 bool rows_aligned(const void* p, int64_t stride, int dtype) {
     return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * static_cast<int64_t>(type_size(dtype)) % 16 == 0);
 }
 int pad_cols(int64_t k) { return static_cast<int>((k + kTileCols - 1) / kTileCols * kTileCols); }
 }  // namespace
 
+constexpr int kFewRows = 512;
+
 hipError_t launch_rows(const NormArgs& a, hipStream_t s) {
     if (a.rows == 0) return hipSuccess;
     const bool vec = a.cols % kElems == 0 && rows_aligned(a.x, a.x_stride, a.dtype) && rows_aligned(a.residual, a.residual_stride, a.dtype) &&
                      rows_aligned(a.h_out, a.h_stride, a.dtype) && rows_aligned(a.values, a.values_stride, a.dtype) &&
                      rows_aligned(a.weight, 0, a.dtype);
-    RowsArgs ra{a, pad_cols(a.cols)};
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(a.rows, 1 << 20)));
+    // Waves a row takes with one run of 512 columns each.  Few rows: as many (up to 16), for their latency; many rows: two or
+    // four runs a wave, whose loads are under way at once.
+    const int kp = pad_cols(a.cols), all = (kp + 511) / 512;
+    int ch = all <= 16 && a.rows <= kFewRows ? 1 : all <= 1 ? 1 : all <= 32 ? 2 : all <= 64 ? 4 : 0;
+    const int waves = ch ? (all + ch - 1) / ch : kLongThreads / 64;
+    const int teams = waves >= 4 ? 1 : 4 / waves;
+    const RowsArgs ra{a, kp, waves};
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((a.rows + teams - 1) / teams, 1 << 20))), block(64 * waves * teams);
     return by_type(a.dtype, [&](auto t) {
         using T = decltype(t);
-        return by_group(a.group, [&](auto g) {
-            return by_bool(vec, [&](auto v) {
-                constexpr int G = decltype(g)::value;
-                constexpr bool V = decltype(v)::value;
-                if (!a.weight) hipLaunchKernelGGL((rows_kernel<T, T, G, false, V>), grid, dim3(256), 0, s, ra);
-                else if (a.weight_dtype == a.dtype) hipLaunchKernelGGL((rows_kernel<T, T, G, true, V>), grid, dim3(256), 0, s, ra);
-                else hipLaunchKernelGGL((rows_kernel<T, float, G, true, V>), grid, dim3(256), 0, s, ra);
-                return hipGetLastError();
-            });
+        return by_bool(vec, [&](auto v) {
+            constexpr bool V = decltype(v)::value;
+            if (ch == 1) hipLaunchKernelGGL((rows_kernel<T, 1, V>), grid, block, 0, s, ra);
+            else if (ch == 2) hipLaunchKernelGGL((rows_kernel<T, 2, V>), grid, block, 0, s, ra);
+            else if (ch == 4) hipLaunchKernelGGL((rows_kernel<T, 4, V>), grid, block, 0, s, ra);
+            else hipLaunchKernelGGL((rows_kernel<T, 0, V>), grid, block, 0, s, ra);
+            return hipGetLastError();
         });
     });
 }
 
 namespace {
+// Matrices of so many rows take four tile rows a workgroup.
 constexpr int kFewWide = 32768;
 
-template <int G, int MT, int R, int NT, int U>
-hipError_t launch_few(const ProductArgs& a, hipStream_t s) {
-    const int kb = pad_cols(a.k) / kTileCols, W = std::min(kb, kFewWaves);
-    const int tiles = (a.n + kTileRows - 1) / kTileRows;
-    hipLaunchKernelGGL((few_kernel<G, MT, R, NT, U>), dim3((tiles + NT - 1) / NT), dim3(64 * W), W * NT * MT * R * 64 * sizeof(float), s, FewArgs{a});
+template <int G, int NT, int U, bool FUSED>
+hipError_t launch_few(const FewArgs& a, int waves, hipStream_t s) {
+    const int tiles = (a.p.n + kTileRows - 1) / kTileRows;
+    hipLaunchKernelGGL((few_kernel<G, NT, U, FUSED>), dim3((tiles + NT - 1) / NT), dim3(64 * waves), 0, s, a);
     return hipGetLastError();
+}
+template <int G, bool FUSED>
+hipError_t few_rows(const FewArgs& a, hipStream_t s) {
+    const int kb = pad_cols(a.p.k) / kTileCols, waves = std::min(kb, kFewWaves), each = (kb + waves - 1) / waves;
+    if constexpr (!FUSED) {
+        if (a.p.n >= kFewWide) return each == 1 ? launch_few<G, 4, 1, FUSED>(a, waves, s) : launch_few<G, 4, 2, FUSED>(a, waves, s);
+    }
+    // tiles of columns a wave takes in a turn: those that leave the fewest of its last turn idle
+    int u = 1;
+    for (int k = 2; k <= 5; ++k)
+        if ((each + k - 1) / k * k <= (each + u - 1) / u * u || u == 1) u = each >= k ? k : u;
+    switch (u) {
+        case 1: return launch_few<G, 1, 1, FUSED>(a, waves, s);
+        case 2: return launch_few<G, 1, 2, FUSED>(a, waves, s);
+        case 3: return launch_few<G, 1, 3, FUSED>(a, waves, s);
+        case 4: return launch_few<G, 1, 4, FUSED>(a, waves, s);
+        default: return launch_few<G, 1, 5, FUSED>(a, waves, s);
+    }
 }
 template <int G, int NT>
 hipError_t launch_batch(const ProductArgs& a, hipStream_t s) {
@@ -714,10 +872,7 @@ hipError_t launch_tiles(const ProductArgs& a, hipStream_t s) {
 }
 template <int G>
 hipError_t product(const ProductArgs& a, hipStream_t s) {
-    if (a.rows <= 4) {
-        if (a.n >= kFewWide) return launch_few<G, 1, 1, 4, 1>(a, s);
-        return launch_few<G, 1, 1, 1, 4>(a, s);
-    }
+    if (a.rows <= kFewTokens) return few_rows<G, false>(FewArgs{a}, s);
 #ifdef VAR
     const int var = std::getenv("VAR") ? std::atoi(std::getenv("VAR")) : 0;
     switch (var) {
@@ -754,6 +909,30 @@ hipError_t launch_product(const ProductArgs& given, hipStream_t s) {
     ProductArgs a = given;
     a.wide = rows_aligned(a.out, a.out_stride, a.dtype) && rows_aligned(a.residual, a.residual_stride, a.dtype);
     return by_group(a.group, [&](auto g) { return product<decltype(g)::value>(a, s); });
+}
+
+// A row that every workgroup norms for itself: not for more workgroups than are resident together (four a CU).
+bool linear_is_fused(int64_t rows, int64_t n, int64_t k) { return rows == 1 && n <= 1024 * kTileRows && k <= kFusedCols; }
+
+hipError_t launch_few(const FewArgs& a, hipStream_t s) {
+    return by_group(a.p.group, [&](auto g) { return few_rows<decltype(g)::value, false>(a, s); });
+}
+
+hipError_t launch_fused(const FewArgs& given, hipStream_t s) {
+    FewArgs a = given;
+    a.vec = a.p.k % kElems == 0 && rows_aligned(a.rows.x, a.rows.x_stride, a.rows.dtype) && rows_aligned(a.rows.weight, 0, a.rows.dtype);
+    return by_group(a.p.group, [&](auto g) { return few_rows<decltype(g)::value, true>(a, s); });
+}
+
+hipError_t launch_linear(const ProductArgs& product, const NormArgs& rows, hipStream_t s) {
+    if (product.rows == 0) return hipSuccess;
+    if (linear_is_fused(product.rows, product.n, product.k)) return launch_fused(FewArgs{product, rows}, s);
+    const hipError_t e = launch_rows(rows, s);
+    if (e != hipSuccess) return e;
+    ProductArgs p = product;
+    p.q = rows.q;
+    p.qscales = rows.scales;
+    return launch_product(p, s);
 }
 
 hipError_t launch_pack(const void* w, int64_t stride, int dtype, int n, int k, int group, void* packed, void* scales, hipStream_t s) {
@@ -953,7 +1132,7 @@ int itts_q4_matmul(const int8_t* q, const float* qscales, int64_t rows, const vo
 }
 
 size_t itts_q4_linear_workspace(int64_t rows, int64_t n, int64_t k, int32_t group) {
-    if (rows < 1 || n < 1 || k < 1 || k > kMaxK || !group_ok(group)) return 0;
+    if (rows < 1 || n < 1 || k < 1 || k > kMaxK || !group_ok(group) || linear_is_fused(rows, n, k)) return 0;
     return codes_bytes(rows, k) + static_cast<size_t>(rows) * (pad_cols(k) / group) * sizeof(float);
 }
 
@@ -974,12 +1153,9 @@ int itts_q4_linear(const void* x, int64_t x_stride, int32_t x_dtype, int64_t row
         need(bytes == 0 || (workspace && workspace_bytes >= bytes), "Workspace too small");
         need(aligned(workspace, 256), "Misaligned workspace");
         int8_t* q = static_cast<int8_t*>(workspace);
-        float* qs = reinterpret_cast<float*>(q + codes_bytes(rows, k));
-        const NormArgs a{x, x_stride, nullptr, 0, norm_weight, weight_dtype, x_dtype, rows, k, eps, group, nullptr, 0, nullptr, 0, q, qs};
-        launched(launch_rows(a, static_cast<hipStream_t>(stream)));
-        p.q = q;
-        p.qscales = qs;
-        launched(launch_product(p, static_cast<hipStream_t>(stream)));
+        float* qs = bytes ? reinterpret_cast<float*>(q + codes_bytes(rows, k)) : nullptr;
+        const NormArgs r{x, x_stride, nullptr, 0, norm_weight, weight_dtype, x_dtype, rows, k, eps, group, nullptr, 0, nullptr, 0, q, qs};
+        launched(launch_linear(p, r, static_cast<hipStream_t>(stream)));
     });
 }
 

@@ -6,7 +6,7 @@
 // added.  So that the codes are a function of the row alone, whatever the launch, the squares are added, and y / s
 // is formed, in 64 bits: v_fma_f64 runs at the rate of v_fma_f32 here, and a row's memory traffic takes longer.
 #pragma once
-#include "common.h"
+#include "q4.h"
 
 namespace itts {
 namespace q4 {
@@ -21,28 +21,86 @@ constexpr int kElems = 8;  // consecutive columns that a lane holds
 __device__ __forceinline__ double join64(float lo, float hi) { return __hiloint2double(__float_as_int(hi), __float_as_int(lo)); }
 __device__ __forceinline__ float lo64(double v) { return __int_as_float(__double2loint(v)); }
 __device__ __forceinline__ float hi64(double v) { return __int_as_float(__double2hiint(v)); }
-__device__ __forceinline__ double lane_x1(double v) { return join64(itts::lane_x1(lo64(v)), itts::lane_x1(hi64(v))); }
-__device__ __forceinline__ double lane_x2(double v) { return join64(itts::lane_x2(lo64(v)), itts::lane_x2(hi64(v))); }
-__device__ __forceinline__ double lane_x4(double v) { return join64(itts::lane_x4(lo64(v)), itts::lane_x4(hi64(v))); }
-__device__ __forceinline__ double lane_x8(double v) { return join64(itts::lane_x8(lo64(v)), itts::lane_x8(hi64(v))); }
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int d = 32; d > 8; d >>= 1) v += __shfl_xor(v, d);
-    v += lane_x8(v);
-    v += lane_x4(v);
-    v += lane_x2(v);
-    return v + lane_x1(v);
+// op of the values of lanes l and l ^ D, in the order of the lanes
+template <int D, class F>
+__device__ __forceinline__ double pair64(double v, F op) {
+    if constexpr (D >= 16) {
+        const uint32_t lo = static_cast<uint32_t>(__double2loint(v)), hi = static_cast<uint32_t>(__double2hiint(v));
+        if constexpr (D == 32) {
+            const auto a = __builtin_amdgcn_permlane32_swap(lo, lo, false, false), b = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+            return op(__hiloint2double(b[0], a[0]), __hiloint2double(b[1], a[1]));
+        } else {
+            const auto a = __builtin_amdgcn_permlane16_swap(lo, lo, false, false), b = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+            return op(__hiloint2double(b[0], a[0]), __hiloint2double(b[1], a[1]));
+        }
+    } else if constexpr (D == 8) {
+        return op(v, join64(lane_x8(lo64(v)), lane_x8(hi64(v))));
+    } else if constexpr (D == 4) {
+        return op(v, join64(lane_x4(lo64(v)), lane_x4(hi64(v))));
+    } else if constexpr (D == 2) {
+        return op(v, join64(lane_x2(lo64(v)), lane_x2(hi64(v))));
+    } else {
+        return op(v, join64(lane_x1(lo64(v)), lane_x1(hi64(v))));
+    }
 }
+__device__ __forceinline__ double add64(double a, double b) { return a + b; }
 // The larger, NaN if one is.
-__device__ __forceinline__ double max_nan(double a, double b) { return a > b || a != a ? a : b; }
-// Over the G / 8 lanes that hold a group.
-template <int G>
-__device__ __forceinline__ double group_max64(double v) {
-    v = max_nan(v, lane_x1(v));
-    v = max_nan(v, lane_x2(v));
-    if constexpr (G >= 64) v = max_nan(v, lane_x4(v));
-    if constexpr (G >= 128) v = max_nan(v, lane_x8(v));
-    return v;
+__device__ __forceinline__ double max64(double a, double b) { return a > b || a != a ? a : b; }
+
+// ------------------------------------------------------------------ a row's squares
+// One order for every kernel: four neighbours one after the other, then pairs of such sums up to blocks of 128
+// columns, then every 64th block one after the other, then pairs of those.
+template <int E>
+__device__ __forceinline__ double lane_squares(const float (&v)[E]) {
+    double s[E / 4];
+#pragma unroll
+    for (int q = 0; q < E / 4; ++q) {
+        s[q] = static_cast<double>(v[4 * q]) * static_cast<double>(v[4 * q]);
+#pragma unroll
+        for (int i = 1; i < 4; ++i) s[q] = fma(static_cast<double>(v[4 * q + i]), static_cast<double>(v[4 * q + i]), s[q]);
+    }
+    if constexpr (E == 8) return s[0] + s[1];
+    else return s[0];
+}
+// Over the 128 / E lanes of a block.
+template <int E>
+__device__ __forceinline__ double block_squares(double s) {
+    s = pair64<1>(s, add64);
+    s = pair64<2>(s, add64);
+    s = pair64<4>(s, add64);
+    s = pair64<8>(s, add64);
+    if constexpr (E == 4) s = pair64<16>(s, add64);
+    return s;
+}
+// Of a row's blocks in LDS; every lane has the sum.
+__device__ __forceinline__ double row_squares(const double* blocks, int count, int lane) {
+    double s = 0.0;
+    for (int b = lane; b < count; b += 64) s += blocks[b];
+    s = pair64<1>(s, add64);
+    s = pair64<2>(s, add64);
+    s = pair64<4>(s, add64);
+    s = pair64<8>(s, add64);
+    s = pair64<16>(s, add64);
+    return pair64<32>(s, add64);
+}
+// 1 / sqrt(v) and 1 / v to a few units of the last place: the instruction's estimate and two Newton steps
+// (a correctly rounded quotient and root take ten times the steps, one after the other).
+__device__ __forceinline__ double inv_sqrt64(double v) {
+    const double e = __builtin_amdgcn_rsq(v);
+    double y = e;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) y = fma(y * 0.5, fma(-v * y, y, 1.0), y);
+    return v > 0.0 && v < __builtin_huge_val() ? y : e;
+}
+__device__ __forceinline__ double inv64(double v) {
+    const double e = __builtin_amdgcn_rcp(v);
+    double y = e;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) y = fma(y, fma(-v, y, 1.0), y);
+    return y;
+}
+__device__ __forceinline__ double inv_rms(double squares, const NormArgs& a) {
+    return inv_sqrt64(squares * inv64(static_cast<double>(a.cols)) + static_cast<double>(a.eps));
 }
 
 // ------------------------------------------------------------------ element types
@@ -56,47 +114,43 @@ __device__ __forceinline__ T from_float(float v) {
     return static_cast<T>(v);
 }
 
-template <class T>
-struct alignas(sizeof(T) * kElems) Pack8 {
-    T v[kElems];
-};
-template <class T>
-struct alignas(16) Part16 {
-    T v[16 / sizeof(T)];
+template <class T, int N>
+struct alignas(sizeof(T) * N) Part {
+    T v[N];
 };
 
-// Eight elements from column c of a row of `cols`, zeros behind its end.  VEC: the row is 16-byte
+// E elements from column c of a row of `cols`, zeros behind its end.  VEC: the row is 16-byte
 // aligned and a multiple of eight columns long.
-template <bool VEC, class T>
-__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t cols, float (&out)[kElems]) {
+template <bool VEC, class T, int E>
+__device__ __forceinline__ void load_row(const T* row, int64_t c, int64_t cols, float (&out)[E]) {
     if constexpr (VEC) {
-        constexpr int P = 16 / sizeof(T);
+        constexpr int P = E * sizeof(T) < 16 ? E : 16 / sizeof(T);
 #pragma unroll
-        for (int i = 0; i < kElems; ++i) out[i] = 0.0f;
+        for (int i = 0; i < E; ++i) out[i] = 0.0f;
         if (c < cols) {
 #pragma unroll
-            for (int k = 0; k < kElems / P; ++k) {
-                const Part16<T> p = *reinterpret_cast<const Part16<T>*>(row + c + k * P);
+            for (int k = 0; k < E / P; ++k) {
+                const Part<T, P> p = *reinterpret_cast<const Part<T, P>*>(row + c + k * P);
 #pragma unroll
                 for (int i = 0; i < P; ++i) out[k * P + i] = to_float(p.v[i]);
             }
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < kElems; ++i) out[i] = c + i < cols ? to_float(row[c + i]) : 0.0f;
+        for (int i = 0; i < E; ++i) out[i] = c + i < cols ? to_float(row[c + i]) : 0.0f;
     }
 }
 template <bool VEC, class T>
-__device__ __forceinline__ void store8(T* row, int64_t c, int64_t cols, const float (&in)[kElems]) {
+__device__ __forceinline__ void store_row(T* row, int64_t c, int64_t cols, const float (&in)[kElems]) {
     if constexpr (VEC) {
         constexpr int P = 16 / sizeof(T);
         if (c < cols) {
 #pragma unroll
             for (int k = 0; k < kElems / P; ++k) {
-                Part16<T> p;
+                Part<T, P> p;
 #pragma unroll
                 for (int i = 0; i < P; ++i) p.v[i] = from_float<T>(in[k * P + i]);
-                *reinterpret_cast<Part16<T>*>(row + c + k * P) = p;
+                *reinterpret_cast<Part<T, P>*>(row + c + k * P) = p;
             }
         }
     } else {
@@ -107,38 +161,42 @@ __device__ __forceinline__ void store8(T* row, int64_t c, int64_t cols, const fl
 }
 
 // ------------------------------------------------------------------ 8-bit codes
-// The codes and the scale of this lane's group, of which it holds the eight values z[i] * inv (z = x or
-// h * weight, exact in 64 bits; inv = 1 or the row's 1 / rms).  inside: the group begins before the row's end.
-template <int G>
-__device__ __forceinline__ float group_codes(const double (&z)[kElems], double inv, bool inside, int8_t (&code)[kElems]) {
+// The codes and the scale of this lane's group of `group` columns, of which it holds the E values z[i] * inv (z = x
+// or h * weight, exact in 64 bits; inv = 1 or the row's 1 / rms).  inside: the group begins before the row's end.
+template <int E>
+__device__ __forceinline__ float group_codes(const double (&z)[E], double inv, int group, bool inside, int8_t (&code)[E]) {
     double top = 0.0, bad = 0.0;
 #pragma unroll
-    for (int i = 0; i < kElems; ++i) {
+    for (int i = 0; i < E; ++i) {
         top = fmax(top, fabs(z[i]));    // (leaves NaN out)
         bad = fma(z[i], 0.0, bad);      // NaN if z[i] is not finite
     }
-    top = group_max64<G>(top + bad);
-    float s = static_cast<float>(top * inv / 127.0);
+    top += bad;
+    top = pair64<1>(top, max64);
+    top = pair64<2>(top, max64);
+    if constexpr (E == 4) top = pair64<4>(top, max64);
+    if (group >= 64) {
+        top = pair64<E == 4 ? 8 : 4>(top, max64);
+        if (group >= 128) top = pair64<E == 4 ? 16 : 8>(top, max64);
+    }
+    float s = static_cast<float>(top * inv * (1.0 / 127.0));
     if (!(s <= 3.402823466e38f)) s = __uint_as_float(0x7fc00000u);
     if (!inside) s = 0.0f;  // (inv may be infinite or NaN)
-    const double c = inv / static_cast<double>(s);
+    const double c = inv * inv64(static_cast<double>(s));
 #pragma unroll
-    for (int i = 0; i < kElems; ++i) {
+    for (int i = 0; i < E; ++i) {
         double t = z[i] * c;
-        // next to a half the product's rounding could decide: the quotient itself does
+        // next to a half the roundings could decide: the quotient itself does
         if (fabs(fabs(t - rint(t)) - 0.5) < 1e-9) t = z[i] * inv / static_cast<double>(s);
         const double r = fmin(fmax(rint(t), -127.0), 127.0);
         code[i] = s > 0.0f ? static_cast<int8_t>(static_cast<int>(r)) : int8_t(0);
     }
     return s;
 }
-__device__ __forceinline__ uint2 pack_codes(const int8_t (&c)[kElems]) {
-    uint2 v = make_uint2(0, 0);
+__device__ __forceinline__ uint32_t four_codes(const int8_t* c) {
+    uint32_t v = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v.x |= static_cast<uint32_t>(static_cast<uint8_t>(c[i])) << (8 * i);
-        v.y |= static_cast<uint32_t>(static_cast<uint8_t>(c[4 + i])) << (8 * i);
-    }
+    for (int i = 0; i < 4; ++i) v |= static_cast<uint32_t>(static_cast<uint8_t>(c[i])) << (8 * i);
     return v;
 }
 
