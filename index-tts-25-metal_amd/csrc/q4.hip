@@ -10,19 +10,17 @@
 namespace itts {
 namespace q4 {
 
-// Elements of a type known at run time, as load_row; vec: as its VEC.
-template <int E>
-__device__ __forceinline__ void load_row_as(const void* row, int64_t c, int64_t cols, int dtype, bool vec, float (&out)[E]) {
-    if (dtype == ITTS_T_F32) {
-        if (vec) load_row<true>(static_cast<const float*>(row), c, cols, out);
-        else load_row<false>(static_cast<const float*>(row), c, cols, out);
-    } else if (dtype == ITTS_T_BF16) {
-        if (vec) load_row<true>(static_cast<const __bf16*>(row), c, cols, out);
-        else load_row<false>(static_cast<const __bf16*>(row), c, cols, out);
-    } else {
-        if (vec) load_row<true>(static_cast<const _Float16*>(row), c, cols, out);
-        else load_row<false>(static_cast<const _Float16*>(row), c, cols, out);
-    }
+// load_raw and floats for a type known at run time.
+template <bool VEC, int E>
+__device__ __forceinline__ void load_raw_as(const void* row, int64_t c, int64_t cols, int dtype, Raw<E>& out) {
+    if (dtype == ITTS_T_F32) load_raw<VEC>(static_cast<const float*>(row), c, cols, out);
+    else load_raw<VEC>(static_cast<const _Float16*>(row), c, cols, out);
+}
+template <bool VEC, int E>
+__device__ __forceinline__ void floats_as(const Raw<E>& in, int dtype, float (&out)[E]) {
+    if (dtype == ITTS_T_F32) floats<VEC, float>(in, out);
+    else if (dtype == ITTS_T_BF16) floats<VEC, __bf16>(in, out);
+    else floats<VEC, _Float16>(in, out);
 }
 
 // ------------------------------------------------------------------ rows to 8 bits
@@ -35,90 +33,89 @@ struct RowsArgs {
 };
 constexpr int kLongThreads = 1024;
 
-template <class T, int CH, bool VEC>
+template <class T, int CH, bool VEC, bool RES>
 __global__ __launch_bounds__(1024) void rows_kernel(RowsArgs ra) {
     const NormArgs& a = ra.a;
     constexpr int N = CH ? CH : 1;
-    constexpr int kBlocks = CH ? 16 * 4 * CH : 64;  // blocks of 128 columns: up to 16 waves of 4 CH
-    __shared__ double blocks[kBlocks];
+    constexpr int kEights = CH ? 1024 * CH : 1024;
+    __shared__ double eights[kEights];
     const int lane = threadIdx.x & 63, waves = ra.waves, teams = blockDim.x / (64 * waves);
     const int team = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6) / waves), tid = threadIdx.x - team * waves * 64;
-    const int step = waves * 64 * kElems, kb = ra.kp / kTileCols, passes = CH ? CH : (ra.kp + step - 1) / step;
-    double* mine = blocks + team * (kBlocks / teams);
+    const int step = waves * 64 * kElems, passes = CH ? CH : (ra.kp + step - 1) / step;
+    const bool norm = a.weight != nullptr;
+    double* mine = eights + team * waves * 64 * N;
     for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * teams; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * teams) {
-        const int64_t r = r0 + team;
-        const bool live = r < a.rows;
+        const int64_t r = r0 + team, cols = r < a.rows ? a.cols : 0;  // (rows behind the last one count as empty)
         const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
-        const T* res = a.residual ? static_cast<const T*>(a.residual) + r * a.residual_stride : nullptr;
+        const T* res = RES ? static_cast<const T*>(a.residual) + r * a.residual_stride : nullptr;
         T* h = a.h_out ? static_cast<T*>(a.h_out) + r * a.h_stride : nullptr;
-        float v[N][kElems], w[N][kElems];
-        // (rows behind the last one count as empty)
-        auto hidden = [&](int64_t c, float (&to)[kElems]) {
-            load_row<VEC>(x, c, live ? a.cols : 0, to);
-            if (res) {
+        Raw<kElems> xr[N], rr[N], wr[N];
+        float v[N][kElems];
+        auto fetch = [&](int64_t c, int i) {
+            load_raw<VEC>(x, c, cols, xr[i]);
+            if constexpr (RES) load_raw<VEC>(res, c, cols, rr[i]);
+        };
+        auto hidden = [&](int i) {
+            floats<VEC, T>(xr[i], v[i]);
+            if constexpr (RES) {
                 float u[kElems];
-                load_row<VEC>(res, c, live ? a.cols : 0, u);
+                floats<VEC, T>(rr[i], u);
 #pragma unroll
-                for (int i = 0; i < kElems; ++i) to[i] = to_float(from_float<T>(to[i] + u[i]));
+                for (int e = 0; e < kElems; ++e) v[i][e] = to_float(from_float<T>(v[i][e] + u[e]));
             }
         };
         if constexpr (CH > 0) {
 #pragma unroll
-            for (int i = 0; i < CH; ++i) hidden(tid * kElems + i * step, v[i]);
-            if (a.weight) {
+            for (int i = 0; i < CH; ++i) fetch(tid * kElems + i * step, i);
+            if (norm) {
 #pragma unroll
-                for (int i = 0; i < CH; ++i) load_row_as(a.weight, tid * kElems + i * step, a.cols, a.weight_dtype, VEC, w[i]);
+                for (int i = 0; i < CH; ++i) load_raw_as<VEC>(a.weight, tid * kElems + i * step, a.cols, a.weight_dtype, wr[i]);
             }
+#pragma unroll
+            for (int i = 0; i < CH; ++i) hidden(i);
         }
         double inv = 1.0;
-        if (a.weight) {
-            double sum = 0.0;
-            for (int i = 0; i < passes; ++i) {
-                if constexpr (CH == 0) {
-                    hidden(tid * kElems + static_cast<int64_t>(i) * step, v[0]);
-                    sum += block_squares<kElems>(lane_squares(v[0]));  // of block tid / 16 + 64 i
-                }
-            }
+        if (norm) {
             if constexpr (CH == 0) {
-                if (tid % 16 == 0) mine[tid / 16] = sum;
+                double sum = 0.0;
+                for (int i = 0; i < passes; ++i) {
+                    fetch(tid * kElems + static_cast<int64_t>(i) * step, 0);
+                    hidden(0);
+                    sum += quad_squares(v[0]) + quad_squares(v[0] + 4);
+                }
+                mine[tid] = sum;
             } else {
 #pragma unroll
-                for (int i = 0; i < CH; ++i) {
-                    const double s = block_squares<kElems>(lane_squares(v[i]));
-                    const int b = (tid + i * waves * 64) / 16;
-                    if (tid % 16 == 0 && b < kb) mine[b] = s;
-                }
+                for (int i = 0; i < CH; ++i) mine[tid + i * waves * 64] = quad_squares(v[i]) + quad_squares(v[i] + 4);
             }
             __syncthreads();
-            inv = inv_rms(row_squares(mine, CH ? kb : 64, lane), a);
+            inv = inv_rms(row_squares(mine, waves * 64 * N, lane), a);  // (zeros behind the row's end)
             __syncthreads();
         }
-        auto codes = [&](int64_t c, float (&hv)[kElems], float (&wv)[kElems]) {
-            if (!live || c >= ra.kp) return;  // (whole groups)
-            if (h) store_row<VEC>(h, c, a.cols, hv);
-            double z[kElems];
-#pragma unroll
-            for (int i = 0; i < kElems; ++i) z[i] = a.weight ? static_cast<double>(hv[i]) * static_cast<double>(wv[i]) : static_cast<double>(hv[i]);
-            int8_t code[kElems];
-            const float s = group_codes(z, inv, a.group, c - c % a.group < a.cols, code);
+        auto codes = [&](int64_t c, int i) {
+            if (cols == 0 || c >= ra.kp) return;  // (whole groups)
+            if (h) store_row<VEC>(h, c, cols, v[i]);
+            float w[kElems], code[kElems];
+            if (norm) floats_as<VEC>(wr[i], a.weight_dtype, w);
+            const float s = group_codes(v[i], w, norm, inv, a.group, c - c % a.group < cols, code);
             *reinterpret_cast<uint2*>(a.q + r * ra.kp + c) = make_uint2(four_codes(code), four_codes(code + 4));
             if (c % a.group == 0) a.scales[r * (ra.kp / a.group) + c / a.group] = s;
             if (a.values) {
-                float u[kElems];
 #pragma unroll
-                for (int i = 0; i < kElems; ++i) u[i] = static_cast<float>(code[i]) * s;
-                store_row<VEC>(static_cast<T*>(a.values) + r * a.values_stride, c, a.cols, u);
+                for (int e = 0; e < kElems; ++e) code[e] *= s;
+                store_row<VEC>(static_cast<T*>(a.values) + r * a.values_stride, c, cols, code);
             }
         };
         if constexpr (CH > 0) {
 #pragma unroll
-            for (int i = 0; i < CH; ++i) codes(tid * kElems + i * step, v[i], w[i]);
+            for (int i = 0; i < CH; ++i) codes(tid * kElems + i * step, i);
         } else {
             for (int i = 0; i < passes; ++i) {
                 const int64_t c = tid * kElems + static_cast<int64_t>(i) * step;
-                hidden(c, v[0]);
-                if (a.weight) load_row_as(a.weight, c, a.cols, a.weight_dtype, VEC, w[0]);
-                codes(c, v[0], w[0]);
+                fetch(c, 0);
+                if (norm) load_raw_as<VEC>(a.weight, c, a.cols, a.weight_dtype, wr[0]);
+                hidden(0);
+                codes(c, 0);
             }
         }
     }
@@ -146,9 +143,12 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     const int64_t row = t / kb * kTileRows + r;
     const int c0 = static_cast<int>(t % kb) * kTileCols + 8 * j;
     const T* src = static_cast<const T*>(a.w) + row * a.stride;
+    Raw<kElems> raw[4];
     float v[4][kElems];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) load_row<VEC>(src, c0 + 32 * b, row < a.n ? a.k : 0, v[b]);
+    for (int b = 0; b < 4; ++b) load_raw<VEC>(src, c0 + 32 * b, row < a.n ? a.k : 0, raw[b]);
+#pragma unroll
+    for (int b = 0; b < 4; ++b) floats<VEC, T>(raw[b], v[b]);
     uint32_t out[4] = {0, 0, 0, 0};
     constexpr int B = G / 32, NG = 4 / B;
     uint16_t sc[NG];
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
     __shared__ __align__(16) uint8_t codes[kBlocks * kFewRow];
     __shared__ float scales[kBlocks * NG];
     __shared__ float sums[kFewWaves * NT * 64];
-    __shared__ double squares[FUSED ? kFusedCols / kTileCols : 1];
+    __shared__ double squares[FUSED ? kFusedCols / kElems : 1];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, quarter = lane >> 4;
     const int W = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kb = (a.k + kTileCols - 1) / kTileCols, tiles = (a.n + kTileRows - 1) / kTileRows;
@@ -385,14 +385,34 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
         const uint8_t* row = static_cast<const uint8_t*>(r.x) + first * r.x_stride * (r.dtype == ITTS_T_F32 ? 4 : 2);
         // four columns a thread, half a wave a block; the first two turns stay in registers between the passes
         constexpr int KEEP = 2;
+        Raw<4> x0[KEEP], w0[KEEP];
         float v0[KEEP][4], g0[KEEP][4];
+        auto request = [&](int p, Raw<4>& v, Raw<4>& g) {
+            if (fa.vec) {
+                load_raw_as<true>(row, p * 4, a.k, r.dtype, v);
+                if (r.weight) load_raw_as<true>(r.weight, p * 4, a.k, r.weight_dtype, g);
+            } else {
+                load_raw_as<false>(row, p * 4, a.k, r.dtype, v);
+                if (r.weight) load_raw_as<false>(r.weight, p * 4, a.k, r.weight_dtype, g);
+            }
+        };
+        auto convert = [&](const Raw<4>& vr, const Raw<4>& gr, float (&v)[4], float (&g)[4]) {
+            if (fa.vec) {
+                floats_as<true>(vr, r.dtype, v);
+                if (r.weight) floats_as<true>(gr, r.weight_dtype, g);
+            } else {
+                floats_as<false>(vr, r.dtype, v);
+                if (r.weight) floats_as<false>(gr, r.weight_dtype, g);
+            }
+        };
         auto fetch = [&](int p, float (&v)[4], float (&g)[4]) {
-            load_row_as(row, p * 4, a.k, r.dtype, fa.vec, v);
-            if (r.weight) load_row_as(r.weight, p * 4, a.k, r.weight_dtype, fa.vec, g);
+            Raw<4> vr, gr;
+            request(p, vr, gr);
+            convert(vr, gr, v, g);
         };
         auto norm = [&](int p, const float (&v)[4]) {
-            const double s = block_squares<4>(lane_squares(v));
-            if ((p & 31) == 0) squares[p >> 5] = s;
+            const double s = pair64<1>(quad_squares(v), add64);
+            if ((p & 1) == 0) squares[p >> 1] = s;
         };
         double inv = 1.0;
         auto quantise = [&](int p, const float (&v)[4], const float (&g)[4]) {
@@ -402,17 +422,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
                 for (int e = 0; e < 4; ++e)
                     if (col + e < a.k) fa.h_out[col + e] = v[e];
             }
-            double z[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z[e] = r.weight ? static_cast<double>(v[e]) * static_cast<double>(g[e]) : static_cast<double>(v[e]);
-            int8_t code[4];
-            const float s = group_codes(z, inv, G, col - col % G < a.k, code);
+            float code[4];
+            const float s = group_codes(v, g, r.weight != nullptr, inv, G, col - col % G < a.k, code);
             *reinterpret_cast<uint32_t*>(codes + (p >> 5) * kFewRow + (p & 31) * 4) = four_codes(code);
             if (col % G == 0) scales[col / G] = s;
         };
 #pragma unroll
         for (int i = 0; i < KEEP; ++i)
-            if (tid + i * T < quads) fetch(tid + i * T, v0[i], g0[i]);
+            if (tid + i * T < quads) request(tid + i * T, x0[i], w0[i]);
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i) convert(x0[i], w0[i], v0[i], g0[i]);
         if (r.weight) {
 #pragma unroll
             for (int i = 0; i < KEEP; ++i)
@@ -423,7 +442,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
                 norm(p, v);
             }
             __syncthreads();
-            if (wave * 64 < quads) inv = inv_rms(row_squares(squares, kb, lane), r);
+            if (wave * 64 < quads) inv = inv_rms(row_squares(squares, kb * (kTileCols / kElems), lane), r);
         }
 #pragma unroll
         for (int i = 0; i < KEEP; ++i)
@@ -795,7 +814,7 @@ hipError_t by_bool(bool b, F&& f) {
     return b ? f(Int<1>()) : f(Int<0>());
 }
 size_t type_size(int dtype) { return dtype == ITTS_T_F32 ? 4 : 2; }
-// Rows that load_row and store_row may take 16 bytes at a time.
+// Rows that load_raw and store_row may take 16 bytes at a time.
 bool rows_aligned(const void* p, int64_t stride, int dtype) {
     return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * static_cast<int64_t>(type_size(dtype)) % 16 == 0);
 }
@@ -820,12 +839,14 @@ hipError_t launch_rows(const NormArgs& a, hipStream_t s) {
     return by_type(a.dtype, [&](auto t) {
         using T = decltype(t);
         return by_bool(vec, [&](auto v) {
-            constexpr bool V = decltype(v)::value;
-            if (ch == 1) hipLaunchKernelGGL((rows_kernel<T, 1, V>), grid, block, 0, s, ra);
-            else if (ch == 2) hipLaunchKernelGGL((rows_kernel<T, 2, V>), grid, block, 0, s, ra);
-            else if (ch == 4) hipLaunchKernelGGL((rows_kernel<T, 4, V>), grid, block, 0, s, ra);
-            else hipLaunchKernelGGL((rows_kernel<T, 0, V>), grid, block, 0, s, ra);
-            return hipGetLastError();
+            return by_bool(a.residual != nullptr, [&](auto res) {
+                constexpr bool V = decltype(v)::value, R = decltype(res)::value;
+                if (ch == 1) hipLaunchKernelGGL((rows_kernel<T, 1, V, R>), grid, block, 0, s, ra);
+                else if (ch == 2) hipLaunchKernelGGL((rows_kernel<T, 2, V, R>), grid, block, 0, s, ra);
+                else if (ch == 4) hipLaunchKernelGGL((rows_kernel<T, 4, V, R>), grid, block, 0, s, ra);
+                else hipLaunchKernelGGL((rows_kernel<T, 0, V, R>), grid, block, 0, s, ra);
+                return hipGetLastError();
+            });
         });
     });
 }

@@ -43,45 +43,48 @@ __device__ __forceinline__ double pair64(double v, F op) {
         return op(v, join64(lane_x1(lo64(v)), lane_x1(hi64(v))));
     }
 }
+template <int D>
+struct Lane {
+    static constexpr int value = D;
+};
+// The value of lane l ^ D.
+template <int D>
+__device__ __forceinline__ float lane_of(float v) {
+    if constexpr (D == 1) return lane_x1(v);
+    else if constexpr (D == 2) return lane_x2(v);
+    else if constexpr (D == 4) return lane_x4(v);
+    else if constexpr (D == 8) return lane_x8(v);
+    else {
+        static_assert(D == 16, "within 32 lanes");
+        return __shfl_xor(v, 16);
+    }
+}
 __device__ __forceinline__ double add64(double a, double b) { return a + b; }
 // The larger, NaN if one is.
 __device__ __forceinline__ double max64(double a, double b) { return a > b || a != a ? a : b; }
 
 // ------------------------------------------------------------------ a row's squares
-// One order for every kernel: four neighbours one after the other, then pairs of such sums up to blocks of 128
-// columns, then every 64th block one after the other, then pairs of those.
-template <int E>
-__device__ __forceinline__ double lane_squares(const float (&v)[E]) {
-    double s[E / 4];
+// One order for every kernel: four neighbours one after the other, two such sums; of these eight-column sums every
+// 64th one after the other, then pairs of those.
+__device__ __forceinline__ double quad_squares(const float* v) {
+    double s = static_cast<double>(v[0]) * static_cast<double>(v[0]);
 #pragma unroll
-    for (int q = 0; q < E / 4; ++q) {
-        s[q] = static_cast<double>(v[4 * q]) * static_cast<double>(v[4 * q]);
-#pragma unroll
-        for (int i = 1; i < 4; ++i) s[q] = fma(static_cast<double>(v[4 * q + i]), static_cast<double>(v[4 * q + i]), s[q]);
-    }
-    if constexpr (E == 8) return s[0] + s[1];
-    else return s[0];
-}
-// Over the 128 / E lanes of a block.
-template <int E>
-__device__ __forceinline__ double block_squares(double s) {
-    s = pair64<1>(s, add64);
-    s = pair64<2>(s, add64);
-    s = pair64<4>(s, add64);
-    s = pair64<8>(s, add64);
-    if constexpr (E == 4) s = pair64<16>(s, add64);
+    for (int i = 1; i < 4; ++i) s = fma(static_cast<double>(v[i]), static_cast<double>(v[i]), s);
     return s;
 }
-// Of a row's blocks in LDS; every lane has the sum.
-__device__ __forceinline__ double row_squares(const double* blocks, int count, int lane) {
-    double s = 0.0;
-    for (int b = lane; b < count; b += 64) s += blocks[b];
+__device__ __forceinline__ double wave_sum64(double s) {
     s = pair64<1>(s, add64);
     s = pair64<2>(s, add64);
     s = pair64<4>(s, add64);
     s = pair64<8>(s, add64);
     s = pair64<16>(s, add64);
     return pair64<32>(s, add64);
+}
+// Of the eight-column sums in LDS; every lane has the result.
+__device__ __forceinline__ double row_squares(const double* eights, int count, int lane) {
+    double s = 0.0;
+    for (int i = lane; i < count; i += 64) s += eights[i];
+    return wave_sum64(s);
 }
 // 1 / sqrt(v) and 1 / v to a few units of the last place: the instruction's estimate and two Newton steps
 // (a correctly rounded quotient and root take ten times the steps, one after the other).
@@ -119,25 +122,45 @@ struct alignas(sizeof(T) * N) Part {
     T v[N];
 };
 
-// E elements from column c of a row of `cols`, zeros behind its end.  VEC: the row is 16-byte
-// aligned and a multiple of eight columns long.
+// E elements from column c of a row of `cols`, as they lie in memory (0 behind the row's end): loads alone, so
+// that several rows' are under way at once.  VEC: the row is 16-byte aligned and a multiple of eight columns long.
+template <int E>
+struct Raw {
+    uint32_t w[E];  // four bytes an element, or (VEC, two-byte types) two elements a word
+};
 template <bool VEC, class T, int E>
-__device__ __forceinline__ void load_row(const T* row, int64_t c, int64_t cols, float (&out)[E]) {
-    if constexpr (VEC) {
-        constexpr int P = E * sizeof(T) < 16 ? E : 16 / sizeof(T);
+__device__ __forceinline__ void load_raw(const T* row, int64_t c, int64_t cols, Raw<E>& out) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) out[i] = 0.0f;
+    for (int i = 0; i < E; ++i) out.w[i] = 0;
+    if constexpr (VEC) {
+        constexpr int words = E * sizeof(T) / 4, P = words < 4 ? words : 4;
         if (c < cols) {
 #pragma unroll
-            for (int k = 0; k < E / P; ++k) {
-                const Part<T, P> p = *reinterpret_cast<const Part<T, P>*>(row + c + k * P);
+            for (int k = 0; k < words / P; ++k) {
+                const Part<uint32_t, P> p = reinterpret_cast<const Part<uint32_t, P>*>(row + c)[k];
 #pragma unroll
-                for (int i = 0; i < P; ++i) out[k * P + i] = to_float(p.v[i]);
+                for (int i = 0; i < P; ++i) out.w[k * P + i] = p.v[i];
             }
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) out[i] = c + i < cols ? to_float(row[c + i]) : 0.0f;
+        for (int i = 0; i < E; ++i)
+            if (c + i < cols) {
+                if constexpr (sizeof(T) == 4) out.w[i] = __builtin_bit_cast(uint32_t, row[c + i]);
+                else out.w[i] = __builtin_bit_cast(uint16_t, row[c + i]);
+            }
+    }
+}
+template <bool VEC, class T, int E>
+__device__ __forceinline__ void floats(const Raw<E>& in, float (&out)[E]) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            out[i] = __uint_as_float(in.w[i]);
+        } else {
+            const uint32_t w = VEC ? in.w[i / 2] >> (16 * (i & 1)) : in.w[i];
+            out[i] = to_float(__builtin_bit_cast(T, static_cast<uint16_t>(w)));
+        }
     }
 }
 template <bool VEC, class T>
@@ -161,43 +184,82 @@ __device__ __forceinline__ void store_row(T* row, int64_t c, int64_t cols, const
 }
 
 // ------------------------------------------------------------------ 8-bit codes
-// The codes and the scale of this lane's group of `group` columns, of which it holds the E values z[i] * inv (z = x
-// or h * weight, exact in 64 bits; inv = 1 or the row's 1 / rms).  inside: the group begins before the row's end.
+// Over the lanes that hold a group of `group` columns, E each.
+template <int E, class T, class F>
+__device__ __forceinline__ T over_group(T v, int group, F step) {
+    v = step(Lane<1>(), v);
+    v = step(Lane<2>(), v);
+    if constexpr (E == 4) v = step(Lane<4>(), v);
+    if (group >= 64) {
+        v = step(Lane<E == 4 ? 8 : 4>(), v);
+        if (group >= 128) v = step(Lane<E == 4 ? 16 : 8>(), v);
+    }
+    return v;
+}
+// The codes q (whole numbers) and the scale of this lane's group: y = v * inv, or v * w * inv with `norm`, of which it
+// holds E values.  inside: the group begins before the row's end.
+// What the scale and a code are is settled in 64 bits, but few values need them.  The scale needs the group's
+// largest product exactly: the largest in FP32 plus the largest remainder (exact by fma) of those that
+// have it.  A code needs them where its quotient in FP32 lies within 1e-4 of a half (product, reciprocal,
+// their products and inv in FP32 are off by at most 127 * 6 * 2^-24 = 4.6e-5).  Groups of zeros, of numbers near the ends of
+// FP32's range or with infinities or NaN take the 64-bit way whole.  All in 64 bits took 66 instead of 30 instructions a value.
 template <int E>
-__device__ __forceinline__ float group_codes(const double (&z)[E], double inv, int group, bool inside, int8_t (&code)[E]) {
-    double top = 0.0, bad = 0.0;
+__device__ __forceinline__ float group_codes(const float (&v)[E], const float (&w)[E], bool norm, double inv, int group, bool inside, float (&q)[E]) {
+    auto exact = [&](int i) { return norm ? static_cast<double>(v[i]) * static_cast<double>(w[i]) : static_cast<double>(v[i]); };
+    auto larger = [](auto d, float x) { return fmaxf(x, lane_of<decltype(d)::value>(x)); };
+    float p[E], top = 0.0f, bad = 0.0f, rest = -INFINITY;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        top = fmax(top, fabs(z[i]));    // (leaves NaN out)
-        bad = fma(z[i], 0.0, bad);      // NaN if z[i] is not finite
+        p[i] = norm ? v[i] * w[i] : v[i];
+        top = fmaxf(top, fabsf(p[i]));
+        bad = __builtin_fmaf(p[i], 0.0f, bad);  // NaN if p[i] is not finite
     }
-    top += bad;
-    top = pair64<1>(top, max64);
-    top = pair64<2>(top, max64);
-    if constexpr (E == 4) top = pair64<4>(top, max64);
-    if (group >= 64) {
-        top = pair64<E == 4 ? 8 : 4>(top, max64);
-        if (group >= 128) top = pair64<E == 4 ? 16 : 8>(top, max64);
+    top = over_group<E>(bad == 0.0f ? top : INFINITY, group, larger);
+    if (norm) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) rest = fmaxf(rest, fabsf(p[i]) == top ? __builtin_fmaf(fabsf(v[i]), fabsf(w[i]), -fabsf(p[i])) : -INFINITY);
+        rest = over_group<E>(rest, group, larger);
+    } else {
+        rest = 0.0f;
     }
-    float s = static_cast<float>(top * inv * (1.0 / 127.0));
+    float s = static_cast<float>((static_cast<double>(top) + static_cast<double>(rest)) * inv * (1.0 / 127.0));
+    if (top >= 1e-25f && top <= 1e38f && s >= 1e-35f && s <= 1e35f && inv <= 1e35) {
+        const float cf = static_cast<float>(inv) * __builtin_amdgcn_rcpf(s);
+        float off = 0.0f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float t = p[i] * cf;
+            q[i] = rintf(t);
+            off = fmaxf(off, fabsf(t - q[i]));
+        }
+        if (off > 0.4999f) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) q[i] = static_cast<float>(rint(exact(i) * inv / static_cast<double>(s)));
+        }
+        return s;
+    }
+    double z = 0.0, none = 0.0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        z = fmax(z, fabs(exact(i)));       // (leaves NaN out)
+        none = fma(exact(i), 0.0, none);   // NaN if it is not finite
+    }
+    z = over_group<E>(z + none, group, [](auto d, double x) { return pair64<decltype(d)::value>(x, max64); });
+    s = static_cast<float>(z * inv * (1.0 / 127.0));
     if (!(s <= 3.402823466e38f)) s = __uint_as_float(0x7fc00000u);
     if (!inside) s = 0.0f;  // (inv may be infinite or NaN)
-    const double c = inv * inv64(static_cast<double>(s));
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        double t = z[i] * c;
-        // next to a half the roundings could decide: the quotient itself does
-        if (fabs(fabs(t - rint(t)) - 0.5) < 1e-9) t = z[i] * inv / static_cast<double>(s);
-        const double r = fmin(fmax(rint(t), -127.0), 127.0);
-        code[i] = s > 0.0f ? static_cast<int8_t>(static_cast<int>(r)) : int8_t(0);
-    }
+    for (int i = 0; i < E; ++i)
+        q[i] = s > 0.0f ? static_cast<float>(fmin(fmax(rint(exact(i) * inv / static_cast<double>(s)), -127.0), 127.0)) : 0.0f;
     return s;
 }
-__device__ __forceinline__ uint32_t four_codes(const int8_t* c) {
-    uint32_t v = 0;
+// Four codes as bytes: adding 1.5 * 2^23 leaves a small whole number in the low bits.
+__device__ __forceinline__ uint32_t four_codes(const float* q) {
+    uint32_t b[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v |= static_cast<uint32_t>(static_cast<uint8_t>(c[i])) << (8 * i);
-    return v;
+    for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(q[i] + 12582912.0f);
+    const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+    return lo | hi;
 }
 
 // ------------------------------------------------------------------ products with packed weights
