@@ -26,9 +26,15 @@ extern "C" {
 
 typedef struct itts_qwen itts_qwen;
 
+/* Flags (no reference counterpart): the layers' matrices, and the head's copy of the embedding,
+ * in 4 bits with a scale per 128 columns, their inputs in 8 bits with scales (itts_ops.h).  Embedding
+ * rows, norms, attention and the cache stay in FP32.  The logits are those of the rounded model. */
+#define ITTS_QWEN_W4 1u
+#define ITTS_QWEN_W4_HEAD 2u
+
 typedef struct {
     uint32_t layers; /* decoder layers; 0 -> 28, the reference's (qwen.cpp:8) */
-    uint32_t flags;  /* reserved, 0 */
+    uint32_t flags;  /* 0 or ITTS_QWEN_W4, ITTS_QWEN_W4_HEAD; the other bits are reserved, 0 */
 } itts_qwen_config;
 
 /* QwenDecoder::QwenDecoder (qwen.cpp:5-15): the tensors by their reference names

@@ -19,8 +19,9 @@ namespace itts25 {
 
 class QwenDecoder {
 public:
+    // flags: those of itts_qwen_config (ITTS_QWEN_W4, ITTS_QWEN_W4_HEAD)
     template <class AnyWeights>
-    explicit QwenDecoder(AnyWeights& weights) : handle_(create(weights)) {}
+    explicit QwenDecoder(AnyWeights& weights, uint32_t flags = 0) : handle_(create(weights, flags)) {}
     ~QwenDecoder();
     QwenDecoder(const QwenDecoder&) = delete;
     QwenDecoder& operator=(const QwenDecoder&) = delete;
@@ -47,18 +48,18 @@ private:
         std::vector<int64_t> shape;
         const std::vector<float>* data;
     };
-    static itts_qwen* create_from_bundle(const itts_bundle* bundle);
-    static itts_qwen* create_from_path(const std::string& bundle_path);
-    static itts_qwen* create_from_tensors(const std::vector<Tensor>& tensors);
+    static itts_qwen* create_from_bundle(const itts_bundle* bundle, uint32_t flags);
+    static itts_qwen* create_from_path(const std::string& bundle_path, uint32_t flags);
+    static itts_qwen* create_from_tensors(const std::vector<Tensor>& tensors, uint32_t flags);
     static std::vector<std::string> tensor_names();
     template <class W>
-    static itts_qwen* create(W& w) {
-        if constexpr (has_handle<W>::value) return create_from_bundle(w.handle());
-        else if constexpr (has_bundle_root<W>::value) return create_from_path(std::string(w.bundle().root()));
+    static itts_qwen* create(W& w, uint32_t flags) {
+        if constexpr (has_handle<W>::value) return create_from_bundle(w.handle(), flags);
+        else if constexpr (has_bundle_root<W>::value) return create_from_path(std::string(w.bundle().root()), flags);
         else {
             std::vector<Tensor> t;
             for (const auto& n : tensor_names()) t.push_back({n, w.info(n).shape, &w.get(n)});
-            return create_from_tensors(t);
+            return create_from_tensors(t, flags);
         }
     }
 };

@@ -34,7 +34,7 @@ std::vector<std::string> QwenDecoder::tensor_names() {
     return n;
 }
 
-itts_qwen* QwenDecoder::create_from_tensors(const std::vector<Tensor>& tensors) {
+itts_qwen* QwenDecoder::create_from_tensors(const std::vector<Tensor>& tensors, uint32_t flags) {
     std::vector<itts_tensor> table;
     for (const auto& t : tensors) {
         itts_tensor e{};
@@ -45,23 +45,26 @@ itts_qwen* QwenDecoder::create_from_tensors(const std::vector<Tensor>& tensors) 
         table.push_back(e);
     }
     itts_qwen* q = nullptr;
-    const int st = itts_qwen_create(table.data(), static_cast<int32_t>(table.size()), nullptr, &q);
+    const itts_qwen_config cfg{0, flags};
+    const int st = itts_qwen_create(table.data(), static_cast<int32_t>(table.size()), &cfg, &q);
     if (st != ITTS_OK) qwen_rethrow(st, itts_qwen_last_error(nullptr));
     return q;
 }
 
-itts_qwen* QwenDecoder::create_from_bundle(const itts_bundle* bundle) {
+itts_qwen* QwenDecoder::create_from_bundle(const itts_bundle* bundle, uint32_t flags) {
     itts_qwen* q = nullptr;
-    const int st = itts_qwen_create_from_bundle(bundle, nullptr, &q);
+    const itts_qwen_config cfg{0, flags};
+    const int st = itts_qwen_create_from_bundle(bundle, &cfg, &q);
     if (st != ITTS_OK) qwen_rethrow(st, itts_qwen_last_error(nullptr));
     return q;
 }
 
-itts_qwen* QwenDecoder::create_from_path(const std::string& bundle_path) {
+itts_qwen* QwenDecoder::create_from_path(const std::string& bundle_path, uint32_t flags) {
     itts_bundle* b = nullptr;
     if (itts_bundle_open(bundle_path.c_str(), 0, &b) != ITTS_OK) throw std::runtime_error(itts_bundle_last_error());
     itts_qwen* q = nullptr;
-    const int st = itts_qwen_create_from_bundle(b, nullptr, &q);
+    const itts_qwen_config cfg{0, flags};
+    const int st = itts_qwen_create_from_bundle(b, &cfg, &q);
     itts_bundle_close(b);  // the decoder holds device copies
     if (st != ITTS_OK) qwen_rethrow(st, itts_qwen_last_error(nullptr));
     return q;

@@ -26,6 +26,10 @@
 // q_argmax_kernel, which picks the token and advances the device state.  The step is
 // captured once as a hipGraph; token, cache length and count live in device QState, so
 // generate() replays it with no per-token host work and polls a flag every 16 tokens.
+// With ITTS_QWEN_W4 the layers' matrices (ITTS_QWEN_W4_HEAD: the head's too) are held in 4 bits with a scale per 128
+// columns (q4.h; 0.24 GB instead of 1.76, 82 MB instead of 622) and the GEMVs become launch_fused: RMSNorm, the
+// row's 8-bit codes and the product in one launch each.  The prefill norms rows to 8-bit codes and multiplies
+// those.  Embedding rows, norms, attention and the cache stay in FP32.
 // Prefill (P ids): embedding rows, RMSNorm rows, split-BF16 GEMMs of prefill.hip (store, residual
 // and SwiGLU epilogues, split K when tiles are few), q_prep_kernel over P rows, causal
 // attention, then the head on the last row.
@@ -40,9 +44,11 @@
 #include <unordered_map>
 #include <vector>
 
+#include "itts_ops.h"
 #include "itts_qwen.h"
 #include "attn_core.h"
 #include "kernels.h"
+#include "q4.h"
 
 namespace itts {
 namespace qwen {
@@ -121,6 +127,7 @@ struct QCausalArgs {
     const float* kc;
     const float* vc;
     uint16_t* out;         // [rows][2048], split operand of o_proj
+    float* out_f32;        // or, with 4-bit weights: as it is
     int rows;
 };
 
@@ -594,6 +601,7 @@ __global__ __launch_bounds__(256) void q_rms_rows_kernel(const float* x, const f
 
 // Causal attention of the prompt rows (qwen_attention, kernels.metal:3119-3129, offset 0): 16 rows
 // of one query head per workgroup (attn_core.h), the last rows (most keys) first.
+template <bool SPLIT>
 __global__ __launch_bounds__(64 * kAttnWaves) void q_causal_attn_kernel(QCausalArgs a) {
     __shared__ AttnLds<kHd> lds;
     const int m0 = (gridDim.x - 1 - blockIdx.x) * kAttnTile, h = blockIdx.y;
@@ -609,7 +617,14 @@ __global__ __launch_bounds__(64 * kAttnWaves) void q_causal_attn_kernel(QCausalA
     attn_merge<kHd>(lds, st, wave, lane, out);
     const int r = tid >> 4, mr = m0 + min(r, nq - 1);
     attn_refine<kHd>(a.q + static_cast<size_t>(mr) * kQ + h * kHd, a.kc + head, a.vc + head, [&] { return mr; }, kScale, r < nq, lane, out);
-    if (r < nq) split_store_piece(a.out, split_off(m0 + r, h * kHd + 8 * (tid & 15), kQ), out);
+    if (r >= nq) return;
+    if constexpr (SPLIT) {
+        split_store_piece(a.out, split_off(m0 + r, h * kHd + 8 * (tid & 15), kQ), out);
+    } else {
+        float4* to = reinterpret_cast<float4*>(a.out_f32 + static_cast<size_t>(m0 + r) * kQ + h * kHd + 8 * (tid & 15));
+        to[0] = make_float4(out[0], out[1], out[2], out[3]);
+        to[1] = make_float4(out[4], out[5], out[6], out[7]);
+    }
 }
 
 #define QWEN_CHECK(x)                                                                                        \
@@ -650,6 +665,24 @@ void gemv(const QGemvArgs& a, hipStream_t s) {
     QWEN_CHECK(hipGetLastError());
 }
 
+// An [n][k] matrix in 4 bits, scales over kQ4Group columns.
+constexpr int kQ4Group = 128;
+struct Q4Matrix {
+    Buf<uint8_t> packed;
+    Buf<uint16_t> scales;
+    int n = 0, k = 0;
+    void pack(const float* w, int rows, int cols, hipStream_t s) {  // w: device, row-major
+        n = rows;
+        k = cols;
+        packed.alloc(itts_q4_packed_bytes(n, k));
+        scales.alloc(itts_q4_scale_count(n, k, kQ4Group));
+        QWEN_CHECK(q4::launch_pack(w, k, ITTS_T_F32, n, k, kQ4Group, packed.p, scales.p, s));
+    }
+};
+struct Q4Layer {
+    Q4Matrix qkv, o, gu, d;
+};
+
 struct Engine {
     std::string last_error;
     int layers = 28;
@@ -663,6 +696,13 @@ struct Engine {
     Buf<float> X, QKV, Qp, ws;
     Buf<uint16_t> Xn, ATT, FF;  // split GEMM operands (gemm_core.h)
     int pcap = 0;
+    // 4-bit weights: the layers' matrices (then `slab` is empty) and the head
+    bool q4_layers = false, q4_head = false;
+    std::vector<Q4Layer> q4;
+    Q4Matrix head;
+    Buf<int8_t> codes, head_codes;   // a prefill's rows in 8 bits ([rows][kF] at most), and the head's row, whose place
+    Buf<float> code_scales, head_scales;  // a captured step keeps
+    Buf<float> ATTf, FFf;
     HostStage* pinned = nullptr;
     hipEvent_t up_done = nullptr;  // the last copy out of pinned->up
     bool up_pending = false;
@@ -686,8 +726,10 @@ struct Engine {
     float* K(int l) const { return kv.p + static_cast<size_t>(2 * l) * kKVH * kCap * kHd; }
     float* Vc(int l) const { return kv.p + static_cast<size_t>(2 * l + 1) * kKVH * kCap * kHd; }
 
-    void create(const std::unordered_map<std::string, Tensor>& t, uint32_t nlayers) {
+    void create(const std::unordered_map<std::string, Tensor>& t, uint32_t nlayers, uint32_t flags) {
         layers = nlayers ? static_cast<int>(nlayers) : 28;
+        q4_layers = flags & ITTS_QWEN_W4;
+        q4_head = flags & ITTS_QWEN_W4_HEAD;
         if (layers < 1 || layers > 28) throw std::invalid_argument("Unsupported Qwen layer count");
         auto get = [&](const std::string& name, std::vector<int64_t> shape) -> const float* {
             auto it = t.find(name);
@@ -728,7 +770,8 @@ struct Engine {
         const char* env = std::getenv("ITTS_QWEN_GRAPHS");
         use_graphs = !(env && std::strcmp(env, "0") == 0);
 
-        slab.alloc(static_cast<size_t>(layers) * kLayerFloats);
+        slab.alloc((q4_layers ? 1 : static_cast<size_t>(layers)) * kLayerFloats);
+        if (q4_layers) q4 = std::vector<Q4Layer>(layers);
         std::vector<float> host(kLayerFloats);
         for (int i = 0; i < layers; ++i) {
             const LW& w = lw[i];
@@ -742,10 +785,24 @@ struct Engine {
                 std::memcpy(hp + kOffGu + size_t(2 * r + 1) * kD, w.u + size_t(r) * kD, sizeof(float) * kD);
             }
             std::memcpy(hp + kOffD, w.d, sizeof(float) * kD * kF);
-            QWEN_CHECK(hipMemcpy(slab.p + static_cast<size_t>(i) * kLayerFloats, hp, sizeof(float) * kLayerFloats, hipMemcpyHostToDevice));
+            QWEN_CHECK(hipMemcpy(slab.p + (q4_layers ? 0 : static_cast<size_t>(i) * kLayerFloats), hp, sizeof(float) * kLayerFloats, hipMemcpyHostToDevice));
+            if (q4_layers) {
+                q4[i].qkv.pack(slab.p, kQkvN, kD, stream);
+                q4[i].o.pack(slab.p + kOffO, kD, kQ, stream);
+                q4[i].gu.pack(slab.p + kOffGu, 2 * kF, kD, stream);
+                q4[i].d.pack(slab.p + kOffD, kD, kF, stream);
+                QWEN_CHECK(hipStreamSynchronize(stream));  // the next layer's copy overwrites the slab
+            }
         }
+        if (q4_layers) slab.reset();
         embed.alloc(static_cast<size_t>(kV) * kD);
         QWEN_CHECK(hipMemcpy(embed.p, E, sizeof(float) * kV * kD, hipMemcpyHostToDevice));
+        if (q4_head) {
+            head.pack(embed.p, kV, kD, stream);
+            QWEN_CHECK(hipStreamSynchronize(stream));
+            head_codes.alloc(kD);
+            head_scales.alloc(kD / kQ4Group);
+        }
         std::vector<float> nh(static_cast<size_t>(layers) * kNormLayer + kD);
         for (int i = 0; i < layers; ++i) {
             float* np = nh.data() + static_cast<size_t>(i) * kNormLayer;
@@ -786,9 +843,17 @@ struct Engine {
         if (P <= pcap) return;
         const int cap = std::max(P, 256);
         X.alloc(static_cast<size_t>(cap) * kD);
-        Xn.alloc(split_elems(cap, kD));
         QKV.alloc(static_cast<size_t>(cap) * kQkvN);
         Qp.alloc(static_cast<size_t>(cap) * kQ);
+        if (q4_layers) {
+            codes.alloc(static_cast<size_t>(cap) * kF);
+            code_scales.alloc(static_cast<size_t>(cap) * (kF / kQ4Group));
+            ATTf.alloc(static_cast<size_t>(cap) * kQ);
+            FFf.alloc(static_cast<size_t>(cap) * kF);
+            pcap = cap;
+            return;
+        }
+        Xn.alloc(split_elems(cap, kD));
         ATT.alloc(split_elems(cap, kQ));
         FF.alloc(split_elems(cap, kF));
         for (auto* b : {&Xn, &ATT, &FF}) QWEN_CHECK(hipMemsetAsync(b->p, 0, b->n * 2, stream));  // padding rows: finite, whatever the memory held
@@ -820,9 +885,69 @@ struct Engine {
         QWEN_CHECK(launch_gemm(g, epi, false, stream));
     }
 
+    // out = (residual +) w times x's rows in 8 bits, normed first with norm_w if that is given; swiglu: n / 2 columns.
+    q4::NormArgs q4_rows(const float* x, int rows, int cols, const float* norm_w) {
+        q4::NormArgs r{};
+        r.x = x;
+        r.x_stride = cols;
+        r.weight = norm_w;
+        r.weight_dtype = r.dtype = ITTS_T_F32;
+        r.rows = rows;
+        r.cols = cols;
+        r.eps = kEps;
+        r.group = kQ4Group;
+        r.q = codes.p;
+        r.scales = code_scales.p;
+        return r;
+    }
+    static q4::ProductArgs q4_product(const Q4Matrix& w, int rows, float* out, const float* residual, bool swiglu) {
+        q4::ProductArgs p{};
+        p.rows = rows;
+        p.packed = w.packed.p;
+        p.wscales = w.scales.p;
+        p.n = w.n;
+        p.k = w.k;
+        p.group = kQ4Group;
+        p.residual = residual;
+        p.swiglu = swiglu;
+        p.dtype = ITTS_T_F32;
+        p.out = out;
+        p.out_stride = p.residual_stride = swiglu ? w.n / 2 : w.n;
+        return p;
+    }
+    void q4_linear(const Q4Matrix& w, const float* x, int rows, const float* norm_w, float* out, const float* residual, bool swiglu) {
+        QWEN_CHECK(q4::launch_linear(q4_product(w, rows, out, residual, swiglu), q4_rows(x, rows, w.k, norm_w), stream));
+    }
+    // The same for a step's row; embedded: x is the embedding table, its row that of the state's token, kept in h.
+    void q4_step(const Q4Matrix& w, const float* x, bool embedded, const float* norm_w, float* out, const float* residual, bool swiglu) {
+        q4::FewArgs a{q4_product(w, 1, out, residual, swiglu), q4_rows(x, 1, w.k, norm_w)};
+        a.active = &st.p->active;
+        if (embedded) {
+            a.token = &st.p->token;
+            a.h_out = h.p;
+        }
+        QWEN_CHECK(q4::launch_fused(a, stream));
+    }
+
     // The head on one row x (RMSNorm with the final weight, logits, workgroup bests) and the
     // token pick advancing the state by `advance` cache rows.
     void enqueue_head(const float* x, uint32_t advance) {
+        if (q4_head) {
+            // (its own launch of the norm: by each of 2374 workgroups it would take longer)
+            q4::NormArgs r = q4_rows(x, 1, kD, norms.p + static_cast<size_t>(layers) * kNormLayer);
+            r.q = head_codes.p;
+            r.scales = head_scales.p;
+            QWEN_CHECK(q4::launch_rows(r, stream));
+            q4::FewArgs f{q4_product(head, 1, logits.p, nullptr, false)};
+            f.p.q = r.q;
+            f.p.qscales = r.scales;
+            f.active = &st.p->active;
+            f.best = best.p;
+            static_assert(kHeadBlocks == kV / 16, "a best per tile row");
+            QWEN_CHECK(q4::launch_few(f, stream));
+            enqueue_argmax(advance);
+            return;
+        }
         QGemvArgs a{};
         a.w = embed.p;
         a.rows = kV;
@@ -832,6 +957,9 @@ struct Engine {
         a.best = best.p;
         a.st = st.p;
         gemv<kD, kHeadRpw, kProRms, kEpiArgmax>(a, stream);
+        enqueue_argmax(advance);
+    }
+    void enqueue_argmax(uint32_t advance) {
         QArgmaxArgs m{best.p, kHeadBlocks, st.p, toks.p, advance};
         hipLaunchKernelGGL(q_argmax_kernel, dim3(1), dim3(1024), 0, stream, m);
         QWEN_CHECK(hipGetLastError());
@@ -844,6 +972,10 @@ struct Engine {
         hipLaunchKernelGGL(q_embed_rows_kernel, dim3(P), dim3(256), 0, s, embed.p, ids.p, X.p);
         QWEN_CHECK(hipGetLastError());
         for (int l = 0; l < layers; ++l) {
+            if (q4_layers) {
+                enqueue_prefill_q4(l, P);
+                continue;
+            }
             const float* w = W(l);
             hipLaunchKernelGGL(q_rms_rows_kernel, dim3(P), dim3(256), 0, s, X.p, N(l) + kNormIn, Xn.p);
             QWEN_CHECK(hipGetLastError());
@@ -851,8 +983,8 @@ struct Engine {
             QPrepArgs pa{QKV.p, P, Qp.p, K(l), Vc(l), N(l) + kNormQ, N(l) + kNormK, inv_freq.p, nullptr};
             hipLaunchKernelGGL(q_prep_kernel, dim3(P, kQH + 2 * kKVH), dim3(64), 0, s, pa);
             QWEN_CHECK(hipGetLastError());
-            QCausalArgs ca{Qp.p, K(l), Vc(l), ATT.p, P};
-            hipLaunchKernelGGL(q_causal_attn_kernel, dim3((P + kAttnTile - 1) / kAttnTile, kQH), dim3(64 * kAttnWaves), 0, s, ca);
+            QCausalArgs ca{Qp.p, K(l), Vc(l), ATT.p, nullptr, P};
+            hipLaunchKernelGGL(q_causal_attn_kernel<true>, dim3((P + kAttnTile - 1) / kAttnTile, kQH), dim3(64 * kAttnWaves), 0, s, ca);
             QWEN_CHECK(hipGetLastError());
             gemm(ATT.p, w + kOffO, P, kD, kQ, X.p, nullptr, kGemmResid);
             hipLaunchKernelGGL(q_rms_rows_kernel, dim3(P), dim3(256), 0, s, X.p, N(l) + kNormPost, Xn.p);
@@ -861,6 +993,20 @@ struct Engine {
             gemm(FF.p, w + kOffD, P, kD, kF, X.p, nullptr, kGemmResid);
         }
         enqueue_head(X.p + static_cast<size_t>(P - 1) * kD, static_cast<uint32_t>(P));
+    }
+
+    void enqueue_prefill_q4(int l, int P) {
+        const Q4Layer& w = q4[l];
+        q4_linear(w.qkv, X.p, P, N(l) + kNormIn, QKV.p, nullptr, false);
+        QPrepArgs pa{QKV.p, P, Qp.p, K(l), Vc(l), N(l) + kNormQ, N(l) + kNormK, inv_freq.p, nullptr};
+        hipLaunchKernelGGL(q_prep_kernel, dim3(P, kQH + 2 * kKVH), dim3(64), 0, stream, pa);
+        QWEN_CHECK(hipGetLastError());
+        QCausalArgs ca{Qp.p, K(l), Vc(l), nullptr, ATTf.p, P};
+        hipLaunchKernelGGL(q_causal_attn_kernel<false>, dim3((P + kAttnTile - 1) / kAttnTile, kQH), dim3(64 * kAttnWaves), 0, stream, ca);
+        QWEN_CHECK(hipGetLastError());
+        q4_linear(w.o, ATTf.p, P, nullptr, X.p, X.p, false);
+        q4_linear(w.gu, X.p, P, N(l) + kNormPost, FFf.p, nullptr, true);
+        q4_linear(w.d, FFf.p, P, nullptr, X.p, X.p, false);
     }
 
     // One decode step for the state's token at row st.cached.
@@ -877,13 +1023,20 @@ struct Engine {
             a.embed = embed.p;
             a.h_out = h.p;
             a.out = qkv.p;
-            if (l == 0) gemv<kD, 2, kProEmbedRms, kEpiStore>(a, s);
+            if (q4_layers) q4_step(q4[l].qkv, l == 0 ? embed.p : h.p, l == 0, N(l) + kNormIn, qkv.p, nullptr, false);
+            else if (l == 0) gemv<kD, 2, kProEmbedRms, kEpiStore>(a, s);
             else gemv<kD, 2, kProRms, kEpiStore>(a, s);
             QAttnArgs aa{qkv.p, K(l), Vc(l), N(l) + kNormQ, N(l) + kNormK, inv_freq.p, part_acc.p, part_ml.p, att.p, st.p};
             hipLaunchKernelGGL(q_attn_kernel, dim3(kAttnGrid), dim3(256), 0, s, aa);
             QWEN_CHECK(hipGetLastError());
             hipLaunchKernelGGL(q_attn_merge_kernel, dim3(kQH), dim3(kHd), 0, s, aa);
             QWEN_CHECK(hipGetLastError());
+            if (q4_layers) {
+                q4_step(q4[l].o, att.p, false, nullptr, h.p, h.p, false);
+                q4_step(q4[l].gu, h.p, false, N(l) + kNormPost, ff.p, nullptr, true);
+                q4_step(q4[l].d, ff.p, false, nullptr, h.p, h.p, false);
+                continue;
+            }
             QGemvArgs o{};
             o.st = st.p;
             o.w = w + kOffO;
@@ -1070,7 +1223,7 @@ int qwen_create(const std::unordered_map<std::string, itts::qwen::Tensor>& t, co
     if (!out) return ITTS_EINVAL;
     *out = nullptr;
     auto q = std::make_unique<itts_qwen>();
-    const int st = qwen_guarded(nullptr, [&] { q->e.create(t, cfg ? cfg->layers : 0); });
+    const int st = qwen_guarded(nullptr, [&] { q->e.create(t, cfg ? cfg->layers : 0, cfg ? cfg->flags : 0); });
     if (st == ITTS_OK) *out = q.release();
     return st;
 }

@@ -775,9 +775,22 @@ QWEN_DID_NOT_STOP = "Qwen did not reach EOS within 1024 generated tokens"
 
 
 class QwenDecoder:
-    """itts25::QwenDecoder (include/itts25/qwen.hpp:5-18, src/qwen.cpp:5-49) on the MI355X."""
+    """itts25::QwenDecoder (include/itts25/qwen.hpp:5-18, src/qwen.cpp:5-49) on the MI355X.
 
-    def __init__(self, weights: Dict[str, np.ndarray], layers: int = QWEN_LAYERS):
+    weight_bits 4: the layers' matrices in 4 bits with a scale per 128 columns and their inputs in 8
+    bits, head_bits 4: the head too (weight_bits unless given)."""
+
+    @staticmethod
+    def _flags(weight_bits: int, head_bits: Optional[int]) -> int:
+        head_bits = weight_bits if head_bits is None else head_bits
+        for bits in (weight_bits, head_bits):
+            if bits not in (4, 32):
+                raise InvalidArgument(f"Qwen weights take 4 or 32 bits, not {bits}")
+        return (1 if weight_bits == 4 else 0) | (2 if head_bits == 4 else 0)
+
+    def __init__(self, weights: Dict[str, np.ndarray], layers: int = QWEN_LAYERS, weight_bits: int = 32, head_bits: Optional[int] = None):
+        self._q = None
+        flags = self._flags(weight_bits, head_bits)
         keep, table = {}, []
         for name, v in weights.items():
             a = keep[name] = np.ascontiguousarray(v, dtype=np.float32)
@@ -785,15 +798,16 @@ class QwenDecoder:
             table.append(_Tensor(name.encode(), a.ctypes.data, shape, a.ndim, 0))
         arr = (_Tensor * max(1, len(table)))(*table)
         self._q = C.c_void_p()
-        st = _lib.itts_qwen_create(arr, len(table), C.byref(_QwenConfig(layers, 0)), C.byref(self._q))
+        st = _lib.itts_qwen_create(arr, len(table), C.byref(_QwenConfig(layers, flags)), C.byref(self._q))
         if st != 0:
             _raise(st, _lib.itts_qwen_last_error(None).decode())
 
     @classmethod
-    def from_bundle(cls, bundle: "Bundle", layers: int = QWEN_LAYERS) -> "QwenDecoder":
+    def from_bundle(cls, bundle: "Bundle", layers: int = QWEN_LAYERS, weight_bits: int = 32, head_bits: Optional[int] = None) -> "QwenDecoder":
+        flags = cls._flags(weight_bits, head_bits)
         self = cls.__new__(cls)
         self._q = C.c_void_p()
-        st = _lib.itts_qwen_create_from_bundle(bundle._b, C.byref(_QwenConfig(layers, 0)), C.byref(self._q))
+        st = _lib.itts_qwen_create_from_bundle(bundle._b, C.byref(_QwenConfig(layers, flags)), C.byref(self._q))
         if st != 0:
             _raise(st, _lib.itts_qwen_last_error(None).decode())
         return self

@@ -163,3 +163,8 @@ def test_the_c_abi_refuses(itts, ops):
         assert unpack(**kw) == -1, kw
     assert lib.itts_q4_packed_bytes(17, 129) == 4 * 1024 and lib.itts_q4_packed_bytes(0, 5) == 0 and lib.itts_q4_packed_bytes(1 << 40, 5) == 0
     assert lib.itts_q4_scale_count(17, 129, 32) == 4 * 64 and lib.itts_q4_scale_count(17, 129, 31) == 0
+
+
+def test_weight_bits(itts):
+    for kw in ({"weight_bits": 8}, {"weight_bits": 4, "head_bits": 16}, {"head_bits": 0}):
+        refused(itts, "4 or 32 bits", itts.QwenDecoder, {}, **kw)
