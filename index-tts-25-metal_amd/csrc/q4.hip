@@ -521,7 +521,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
 // bytes) and their scales go through LDS of its own, whole cache lines at a time: as operands straight from
 // memory, 8 bytes a lane from 16 rows, they took longer than the weights (18.7 -> 8.7 us for 16 x 10240 x 5120).
 constexpr int kCodeRow16 = kTileCols + 8;  // 16 rows' pieces of 8 bytes lie in 32 different banks
-template <int G, int NT>
+template <int G, int NT, int U>
 __global__ __launch_bounds__(64 * kFewWaves) void batch_kernel(ProductArgs a) {
     constexpr int NG = 128 / G, kStage = 16 * kCodeRow16 + NG * 16 * 4, S = NT * 4;
     constexpr int kSums = kFewWaves * S * 256, kCodes = kFewWaves * kStage;
@@ -536,7 +536,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void batch_kernel(ProductArgs a) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) xg[i] = a.q + static_cast<int64_t>(min(8 * i + (lane >> 3), a.rows - 1)) * kb * kTileCols + 16 * (lane & 7);
     const int token_g = lane / NG, g_of = lane % NG;  // lanes under 16 NG fetch a scale each
-    const float* sg = a.qscales + static_cast<int64_t>(min(min(token_g, 15), a.rows - 1)) * kb * NG + g_of;
+    const float* sg = a.qscales + static_cast<int64_t>(min(token_g, a.rows - 1)) * kb * NG + g_of;
     const uint8_t* w[NT];
     const uint16_t* ws[NT];
 #pragma unroll
@@ -545,56 +545,54 @@ __global__ __launch_bounds__(64 * kFewWaves) void batch_kernel(ProductArgs a) {
         w[i] = a.packed + row * kTileBytes + lane * 16;
         ws[i] = a.wscales + (row * kTileRows + c) * NG;
     }
-    u32x4 xr[2], wr[NT];
-    float sr = 0.0f;
-    uint16_t wsr[NT][NG];
-    auto fetch = [&](int b) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) xr[i] = *reinterpret_cast<const u32x4*>(xg[i] + b * kTileCols);
-        sr = sg[b * NG];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            wr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(w[i] + static_cast<int64_t>(b) * kTileBytes));
-#pragma unroll
-            for (int g = 0; g < NG; ++g) wsr[i][g] = ws[i][static_cast<int64_t>(b) * kTileRows * NG + g];
-        }
-    };
     float acc[NT][4] = {};
-    if (wave < kb) fetch(wave);
-    for (int b = wave; b < kb; b += W) {
+    for (int b0 = wave; b0 < kb; b0 += W * U) {
+        u32x4 xr[U][2], wr[U][NT];
+        float sr[U];
+        uint16_t wsr[U][NT][NG];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            uint8_t* at = mine + (8 * i + (lane >> 3)) * kCodeRow16 + 16 * (lane & 7);
-            *reinterpret_cast<uint2*>(at) = make_uint2(xr[i][0], xr[i][1]);
-            *reinterpret_cast<uint2*>(at + 8) = make_uint2(xr[i][2], xr[i][3]);
+        for (int u = 0; u < U; ++u) {
+            const int b = min(b0 + u * W, kb - 1);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) xr[u][i] = *reinterpret_cast<const u32x4*>(xg[i] + b * kTileCols);
+            sr[u] = lane < 16 * NG ? sg[b * NG] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                wr[u][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(w[i] + static_cast<int64_t>(b) * kTileBytes));
+#pragma unroll
+                for (int g = 0; g < NG; ++g) wsr[u][i][g] = ws[i][static_cast<int64_t>(b) * kTileRows * NG + g];
+            }
         }
-        if (lane < 16 * NG) *reinterpret_cast<float*>(mine + 16 * kCodeRow16 + (g_of * 16 + token_g) * 4) = sr;
-        u32x4 wc[NT];
-        float sc[NT][NG];
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            wc[i] = wr[i];
+        for (int u = 0; u < U; ++u) {
+            if (b0 + u * W >= kb) break;
+            wave_sync();
 #pragma unroll
-            for (int g = 0; g < NG; ++g) sc[i][g] = weight_scale(wsr[i][g]);
-        }
-        wave_sync();
-        const TokenCodes xc = token_codes(reinterpret_cast<const int8_t*>(mine) + c * kCodeRow16, lane);
-        float xs[NG][4];
+            for (int i = 0; i < 2; ++i) {
+                uint8_t* at = mine + (8 * i + (lane >> 3)) * kCodeRow16 + 16 * (lane & 7);
+                *reinterpret_cast<uint2*>(at) = make_uint2(xr[u][i][0], xr[u][i][1]);
+                *reinterpret_cast<uint2*>(at + 8) = make_uint2(xr[u][i][2], xr[u][i][3]);
+            }
+            if (lane < 16 * NG) *reinterpret_cast<float*>(mine + 16 * kCodeRow16 + (g_of * 16 + token_g) * 4) = sr[u];
+            wave_sync();
+            const TokenCodes xc = token_codes(reinterpret_cast<const int8_t*>(mine) + c * kCodeRow16, lane);
+            float xs[NG][4];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const float4 v = *reinterpret_cast<const float4*>(mine + 16 * kCodeRow16 + (g * 16 + 4 * quarter) * 4);
-            xs[g][0] = v.x, xs[g][1] = v.y, xs[g][2] = v.z, xs[g][3] = v.w;
-        }
-        wave_sync();
-        if (b + W < kb) fetch(b + W);
+            for (int g = 0; g < NG; ++g) {
+                const float4 v = *reinterpret_cast<const float4*>(mine + 16 * kCodeRow16 + (g * 16 + 4 * quarter) * 4);
+                xs[g][0] = v.x, xs[g][1] = v.y, xs[g][2] = v.z, xs[g][3] = v.w;
+            }
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            i32x4 f[NG];
-            tile_product<G>(xc, wc[i], f);
+            for (int i = 0; i < NT; ++i) {
+                i32x4 f[NG];
+                tile_product<G>(xc, wr[u][i], f);
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
+                for (int g = 0; g < NG; ++g) {
+                    const float s = weight_scale(wsr[u][i][g]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[i][r] = __builtin_fmaf(static_cast<float>(f[g][r]), xs[g][r] * sc[i][g], acc[i][r]);
+                    for (int r = 0; r < 4; ++r) acc[i][r] = __builtin_fmaf(static_cast<float>(f[g][r]), xs[g][r] * s, acc[i][r]);
+                }
+            }
         }
     }
     __syncthreads();
@@ -643,46 +641,51 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void tiles_kernel(ProductArgs a)
     const int mblocks = (a.rows + BM - 1) / BM;
     const int m0 = blockIdx.x % mblocks * BM, n0 = blockIdx.x / mblocks * BN;
 
-    const int8_t* xg[CH];
-    int xl[CH];
+    // places relative to the block's first row, in 32 bits: loads take a uniform address and these
+    const int64_t row_bytes = static_cast<int64_t>(kb) * kTileCols, tile_bytes = static_cast<int64_t>(kb) * kTileBytes;
+    const int8_t* const x0 = a.q + m0 * row_bytes;
+    const float* const s0 = a.qscales + static_cast<int64_t>(m0) * kb * NG;
+    const uint8_t* const w0 = a.packed + n0 / 16 * tile_bytes;
+    const uint16_t* const ws0 = a.wscales + static_cast<int64_t>(n0 / 16) * kb * kTileRows * NG;
+    uint32_t xo[CH], so[SC], wo[NT], wso[NT];
+    int xl[CH], sl[SC];
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         const int p = i * TG + tg, r = p >> 3, q = p & 7;
-        xg[i] = a.q + static_cast<int64_t>(min(m0 + r, a.rows - 1)) * kb * kTileCols + 16 * q;
+        xo[i] = static_cast<uint32_t>(min(r, a.rows - 1 - m0)) * static_cast<uint32_t>(row_bytes) + 16 * q;
         xl[i] = r * kCodeRow + 16 * q;
     }
-    const float* sg[SC];
-    int sl[SC];
 #pragma unroll
     for (int i = 0; i < SC; ++i) {
         const int p = min(i * TG + tg, BM * NG - 1), r = p / NG, g = p % NG;
-        sg[i] = a.qscales + static_cast<int64_t>(min(m0 + r, a.rows - 1)) * kb * NG + g;
+        so[i] = static_cast<uint32_t>(min(r, a.rows - 1 - m0)) * static_cast<uint32_t>(kb * NG) + g;
         sl[i] = BM * kCodeRow + (g * BM + r) * 4;
     }
-    const uint8_t* w[NT];
-    const uint16_t* ws[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-        const int64_t row = static_cast<int64_t>(min(n0 / 16 + (wn * NT + i) * 2 + (c >> 4), tiles - 1)) * kb;
-        w[i] = a.packed + row * kTileBytes + (32 * half + (c & 15)) * 16;
-        ws[i] = a.wscales + (row * kTileRows + (c & 15)) * NG;
+        const uint32_t tile = static_cast<uint32_t>(min((wn * NT + i) * 2 + (c >> 4), tiles - 1 - n0 / 16));
+        wo[i] = tile * static_cast<uint32_t>(tile_bytes) + (32 * half + (c & 15)) * 16;
+        wso[i] = (tile * static_cast<uint32_t>(kb) * kTileRows + (c & 15)) * NG;
     }
     u32x4 xr[CH], wr[NT][2];
     float sr[SC];
     uint16_t wsr[NT][NG];
     auto fetch = [&](int step) {
         const int b = min(step * WK + wk, kb - 1);
+        const int8_t* const xb = x0 + b * kTileCols;
+        const float* const sb = s0 + b * NG;
+        const uint8_t* const wb = w0 + static_cast<int64_t>(b) * kTileBytes;
+        const uint16_t* const wsb = ws0 + static_cast<int64_t>(b) * kTileRows * NG;
 #pragma unroll
-        for (int i = 0; i < CH; ++i) xr[i] = *reinterpret_cast<const u32x4*>(xg[i] + b * kTileCols);
+        for (int i = 0; i < CH; ++i) xr[i] = *reinterpret_cast<const u32x4*>(xb + xo[i]);
 #pragma unroll
-        for (int i = 0; i < SC; ++i) sr[i] = sg[i][b * NG];
+        for (int i = 0; i < SC; ++i) sr[i] = sb[so[i]];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            const uint8_t* at = w[i] + static_cast<int64_t>(b) * kTileBytes;
-            wr[i][0] = *reinterpret_cast<const u32x4*>(at);
-            wr[i][1] = *reinterpret_cast<const u32x4*>(at + 256);
+            wr[i][0] = *reinterpret_cast<const u32x4*>(wb + wo[i]);
+            wr[i][1] = *reinterpret_cast<const u32x4*>(wb + wo[i] + 256);
 #pragma unroll
-            for (int g = 0; g < NG; ++g) wsr[i][g] = ws[i][static_cast<int64_t>(b) * kTileRows * NG + g];
+            for (int g = 0; g < NG; ++g) wsr[i][g] = wsb[wso[i] + g];
         }
     };
     auto stage = [&](int step) {
@@ -715,7 +718,17 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void tiles_kernel(ProductArgs a)
             for (int t = 0; t < MT; ++t)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) xc[t][q] = *reinterpret_cast<const i32x4*>(at + ((wm * MT + t) * 32 + c) * kCodeRow + 32 * q + 16 * half);
+            // the tokens' scales, ahead of their use where they fit the registers
             const uint8_t* xs = at + BM * kCodeRow + (wm * MT * 32 + 4 * half) * 4;
+            constexpr bool AHEAD = NG == 1 && MT <= 2;
+            auto token_scales = [&](int t, int g, int q) { return *reinterpret_cast<const float4*>(xs + (g * BM + t * 32 + 8 * q) * 4); };
+            float4 xa[AHEAD ? MT * NG : 1][4];
+            if constexpr (AHEAD) {
+#pragma unroll
+                for (int j = 0; j < MT * NG; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) xa[j][q] = token_scales(j / NG, j % NG, q);
+            }
             // the products of one block of 32 x 32 and group are under way while those of the one before are scaled
             i32x16 f[2];
             auto multiply = [&](int i, int t, int g, i32x16& to) {
@@ -736,7 +749,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK) void tiles_kernel(ProductArgs a)
             auto scale = [&](int i, int t, int g, const i32x16& from) {
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const float4 v = *reinterpret_cast<const float4*>(xs + (g * BM + t * 32 + 8 * q) * 4);
+                    const float4 v = AHEAD ? xa[AHEAD ? t * NG + g : 0][q] : token_scales(t, g, q);
                     const float x4[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
@@ -852,8 +865,18 @@ hipError_t launch_rows(const NormArgs& a, hipStream_t s) {
 }
 
 namespace {
-// Matrices of so many rows take four tile rows a workgroup.
-constexpr int kFewWide = 32768;
+// Matrices of so many rows take four tile rows a workgroup, which then reads the codes once for the four (16 rows x
+// 16384 x 8192: 15.2 us against 18.9; x 10240 x 5120: 9.5 against 10.4, but 8 rows 9.0 against 8.6).
+constexpr int kFewWide = 32768, kBatchWide = 16384;
+
+// Tiles of columns that a wave takes in a turn, of `each` in all: those that leave the fewest of its last turn
+// idle, the more the better.
+int turn_tiles(int each) {
+    int u = 1;
+    for (int k = 2; k <= std::min(each, 5); ++k)
+        if ((each + k - 1) / k * k <= (each + u - 1) / u * u || u == 1) u = k;
+    return u;
+}
 
 template <int G, int NT, int U, bool FUSED>
 hipError_t launch_few(const FewArgs& a, int waves, hipStream_t s) {
@@ -867,11 +890,7 @@ hipError_t few_rows(const FewArgs& a, hipStream_t s) {
     if constexpr (!FUSED) {
         if (a.p.n >= kFewWide) return each == 1 ? launch_few<G, 4, 1, FUSED>(a, waves, s) : launch_few<G, 4, 2, FUSED>(a, waves, s);
     }
-    // tiles of columns a wave takes in a turn: those that leave the fewest of its last turn idle
-    int u = 1;
-    for (int k = 2; k <= 5; ++k)
-        if ((each + k - 1) / k * k <= (each + u - 1) / u * u || u == 1) u = each >= k ? k : u;
-    switch (u) {
+    switch (turn_tiles(each)) {
         case 1: return launch_few<G, 1, 1, FUSED>(a, waves, s);
         case 2: return launch_few<G, 1, 2, FUSED>(a, waves, s);
         case 3: return launch_few<G, 1, 3, FUSED>(a, waves, s);
@@ -879,11 +898,23 @@ hipError_t few_rows(const FewArgs& a, hipStream_t s) {
         default: return launch_few<G, 1, 5, FUSED>(a, waves, s);
     }
 }
-template <int G, int NT>
-hipError_t launch_batch(const ProductArgs& a, hipStream_t s) {
-    const int kb = pad_cols(a.k) / kTileCols, tiles = (a.n + kTileRows - 1) / kTileRows;
-    hipLaunchKernelGGL((batch_kernel<G, NT>), dim3((tiles + NT - 1) / NT), dim3(64 * std::min(kb, kFewWaves)), 0, s, a);
+template <int G, int NT, int U>
+hipError_t launch_batch(const ProductArgs& a, int waves, hipStream_t s) {
+    const int tiles = (a.n + kTileRows - 1) / kTileRows;
+    hipLaunchKernelGGL((batch_kernel<G, NT, U>), dim3((tiles + NT - 1) / NT), dim3(64 * waves), 0, s, a);
     return hipGetLastError();
+}
+template <int G>
+hipError_t batch_rows(const ProductArgs& a, hipStream_t s) {
+    const int kb = pad_cols(a.k) / kTileCols, waves = std::min(kb, kFewWaves), each = (kb + waves - 1) / waves;
+    if (a.n >= kBatchWide) return launch_batch<G, 4, 1>(a, waves, s);
+    switch (turn_tiles(each)) {
+        case 1: return launch_batch<G, 1, 1>(a, waves, s);
+        case 2: return launch_batch<G, 1, 2>(a, waves, s);
+        case 3: return launch_batch<G, 1, 3>(a, waves, s);
+        case 4: return launch_batch<G, 1, 4>(a, waves, s);
+        default: return launch_batch<G, 1, 5>(a, waves, s);
+    }
 }
 template <int G, int WM, int WN, int WK, int MT, int NT>
 hipError_t launch_tiles(const ProductArgs& a, hipStream_t s) {
@@ -897,31 +928,27 @@ hipError_t product(const ProductArgs& a, hipStream_t s) {
 #ifdef VAR
     const int var = std::getenv("VAR") ? std::atoi(std::getenv("VAR")) : 0;
     switch (var) {
-        case 1: return launch_batch<G, 1>(a, s);
-        case 2: return launch_batch<G, 2>(a, s);
-        case 3: return launch_batch<G, 4>(a, s);
-        case 4: return launch_tiles<G, 1, 1, 8, 1, 1>(a, s);
-        case 5: return launch_tiles<G, 1, 1, 4, 1, 1>(a, s);
-        case 6: return launch_tiles<G, 1, 2, 4, 1, 1>(a, s);
-        case 7: return launch_tiles<G, 1, 4, 2, 1, 1>(a, s);
-        case 8: return launch_tiles<G, 1, 4, 1, 1, 1>(a, s);
-        case 9: return launch_tiles<G, 2, 1, 4, 1, 1>(a, s);
-        case 10: return launch_tiles<G, 2, 2, 2, 1, 1>(a, s);
-        case 11: return launch_tiles<G, 2, 2, 1, 1, 1>(a, s);
-        case 12: return launch_tiles<G, 1, 4, 1, 2, 1>(a, s);
-        case 13: return launch_tiles<G, 2, 2, 1, 2, 1>(a, s);
-        case 14: return launch_tiles<G, 2, 2, 1, 2, 2>(a, s);
-        case 15: return launch_tiles<G, 2, 4, 1, 2, 1>(a, s);
-        case 16: return launch_tiles<G, 2, 2, 2, 2, 1>(a, s);
-        case 17: return launch_tiles<G, 1, 4, 1, 4, 1>(a, s);
-        case 18: return launch_tiles<G, 4, 2, 1, 1, 1>(a, s);
-        case 19: return launch_tiles<G, 2, 4, 1, 2, 2>(a, s);
+        case 1: return launch_batch<G, 1, 1>(a, std::min(8, (a.k + 127) / 128), s);
+        case 2: return launch_batch<G, 1, 2>(a, std::min(8, (a.k + 127) / 128), s);
+        case 3: return launch_batch<G, 1, 5>(a, std::min(8, (a.k + 127) / 128), s);
+        case 4: return launch_batch<G, 2, 1>(a, std::min(8, (a.k + 127) / 128), s);
+        case 5: return launch_batch<G, 4, 1>(a, std::min(8, (a.k + 127) / 128), s);
+        case 6: return launch_batch<G, 2, 5>(a, std::min(8, (a.k + 127) / 128), s);
+        case 7: return launch_batch<G, 2, 3>(a, std::min(8, (a.k + 127) / 128), s);
     }
 #endif
-    if (a.rows <= 16) return launch_batch<G, 1>(a, s);
-    if (a.rows <= 32) return launch_tiles<G, 1, 1, 8, 1, 1>(a, s);
-    if (a.rows <= 64) return launch_tiles<G, 2, 1, 4, 1, 1>(a, s);
-    return launch_tiles<G, 2, 2, 1, 2, 1>(a, s);
+    if (a.rows <= 16) return batch_rows<G>(a, s);
+    // Workgroups of 64 x 128 (one wave 64 x 32: the fewest LDS and memory reads a product) where two a CU come of
+    // them; else of 64 x 64, nearly as many; else smaller blocks whose waves share the columns, for the latency of
+    // their turns.  Measured (us; 64 x 128, 64 x 64, 32 x 64 by 4, 32 x 32 by 8): 1024 x 4096 x 4096 33 39 - -;
+    // 512 x 6144 x 1024 12.6 12.1 - -; 155 x 10240 x 1280 12.0 10.5 13.6 -; 256 x 4096 x 4096 in groups of 64 34 26
+    // 16.8 -; 64 x 10240 x 5120 - - 15.3 16.9; 64 x 1024 x 2048 - - 6.3 4.9; 32 x 151936 x 1024 (32 x 128) 23 - 29 36.
+    const auto blocks = [&](int bm, int bn) { return static_cast<int64_t>((a.rows + bm - 1) / bm) * ((a.n + bn - 1) / bn); };
+    if (a.rows <= 32 && blocks(32, 128) >= 512) return launch_tiles<G, 1, 4, 1, 1, 1>(a, s);
+    if (blocks(64, 128) >= 512) return launch_tiles<G, 1, 4, 1, 2, 1>(a, s);
+    if (blocks(64, 64) >= 448) return launch_tiles<G, 2, 2, 1, 1, 1>(a, s);
+    if (blocks(32, 32) <= 512) return launch_tiles<G, 1, 1, 8, 1, 1>(a, s);
+    return launch_tiles<G, 1, 2, 4, 1, 1>(a, s);
 }
 }  // namespace
 
