@@ -12,7 +12,7 @@ namespace q4 {
 
 // load_raw and floats for a type known at run time.
 template <bool VEC, int E>
-__device__ __forceinline__ void load_raw_as(const void* row, int64_t c, int64_t cols, int dtype, Raw<E>& out) {
+__device__ __forceinline__ void load_raw_as(const void* row, uint32_t c, uint32_t cols, int dtype, Raw<E>& out) {
     if (dtype == ITTS_T_F32) load_raw<VEC>(static_cast<const float*>(row), c, cols, out);
     else load_raw<VEC>(static_cast<const _Float16*>(row), c, cols, out);
 }
@@ -23,13 +23,19 @@ __device__ __forceinline__ void floats_as(const Raw<E>& in, int dtype, float (&o
     else floats<VEC, _Float16>(in, out);
 }
 
+// Orders a wave's LDS accesses before and after it.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // ------------------------------------------------------------------ rows to 8 bits
 // Bound by memory: every element is read once.  A team of waves owns a row and keeps it in registers between the
 // two passes, CH runs of eight columns a lane; the norm's weights are requested with the row.  CH = 0: rows
 // longer than that, by 1024 threads, which read h (or x) again.
 struct RowsArgs {
     NormArgs a;
-    int kp, waves;  // padded columns; waves of a team
+    int kp, waves, shift;  // padded columns; waves of a team; log2 of the group
 };
 constexpr int kLongThreads = 1024;
 
@@ -44,42 +50,62 @@ __global__ __launch_bounds__(1024) void rows_kernel(RowsArgs ra) {
     const int step = waves * 64 * kElems, passes = CH ? CH : (ra.kp + step - 1) / step;
     const bool norm = a.weight != nullptr;
     double* mine = eights + team * waves * 64 * N;
-    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * teams; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * teams) {
-        const int64_t r = r0 + team, cols = r < a.rows ? a.cols : 0;  // (rows behind the last one count as empty)
-        const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
-        const T* res = RES ? static_cast<const T*>(a.residual) + r * a.residual_stride : nullptr;
+    Raw<kElems> xr[N], rr[N], wr[N];
+    float v[N][kElems];
+    // (rows behind the last one count as empty)
+    auto width = [&](int64_t r) { return r < a.rows ? static_cast<uint32_t>(a.cols) : 0u; };
+    auto fetch = [&](int64_t r, uint32_t c, int i) {
+        load_raw<VEC>(static_cast<const T*>(a.x) + r * a.x_stride, c, width(r), xr[i]);
+        if constexpr (RES) load_raw<VEC>(static_cast<const T*>(a.residual) + r * a.residual_stride, c, width(r), rr[i]);
+    };
+    auto hidden = [&](int i) {
+        floats<VEC, T>(xr[i], v[i]);
+        if constexpr (RES) {
+            float u[kElems];
+            floats<VEC, T>(rr[i], u);
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) v[i][e] = to_float(from_float<T>(v[i][e] + u[e]));
+        }
+    };
+    const int64_t each = static_cast<int64_t>(gridDim.x) * teams;
+    int64_t r0 = static_cast<int64_t>(blockIdx.x) * teams;
+    // Of one run a lane: the next row's loads are under way while this one is worked on (more do not fit the registers).
+    constexpr bool NEXT = CH == 1;
+    auto begin = [&](int64_t r) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) fetch(r, tid * kElems + i * step, i);
+    };
+    auto weights = [&] {
+        if (norm) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) load_raw_as<VEC>(a.weight, tid * kElems + i * step, a.cols, a.weight_dtype, wr[i]);
+        }
+    };
+    if constexpr (NEXT) {
+        begin(r0 + team);
+        weights();
+    }
+    for (; r0 < a.rows; r0 += each) {
+        const int64_t r = r0 + team;
+        const uint32_t cols = width(r);
         T* h = a.h_out ? static_cast<T*>(a.h_out) + r * a.h_stride : nullptr;
-        Raw<kElems> xr[N], rr[N], wr[N];
-        float v[N][kElems];
-        auto fetch = [&](int64_t c, int i) {
-            load_raw<VEC>(x, c, cols, xr[i]);
-            if constexpr (RES) load_raw<VEC>(res, c, cols, rr[i]);
-        };
-        auto hidden = [&](int i) {
-            floats<VEC, T>(xr[i], v[i]);
-            if constexpr (RES) {
-                float u[kElems];
-                floats<VEC, T>(rr[i], u);
-#pragma unroll
-                for (int e = 0; e < kElems; ++e) v[i][e] = to_float(from_float<T>(v[i][e] + u[e]));
-            }
-        };
         if constexpr (CH > 0) {
-#pragma unroll
-            for (int i = 0; i < CH; ++i) fetch(tid * kElems + i * step, i);
-            if (norm) {
-#pragma unroll
-                for (int i = 0; i < CH; ++i) load_raw_as<VEC>(a.weight, tid * kElems + i * step, a.cols, a.weight_dtype, wr[i]);
+            if constexpr (!NEXT) {
+                begin(r);
+                weights();
             }
 #pragma unroll
             for (int i = 0; i < CH; ++i) hidden(i);
+            if constexpr (NEXT) {
+                if (r0 + each < a.rows) begin(r + each);
+            }
         }
         double inv = 1.0;
         if (norm) {
             if constexpr (CH == 0) {
                 double sum = 0.0;
                 for (int i = 0; i < passes; ++i) {
-                    fetch(tid * kElems + static_cast<int64_t>(i) * step, 0);
+                    fetch(r, tid * kElems + i * step, 0);
                     hidden(0);
                     sum += quad_squares(v[0]) + quad_squares(v[0] + 4);
                 }
@@ -92,14 +118,14 @@ __global__ __launch_bounds__(1024) void rows_kernel(RowsArgs ra) {
             inv = inv_rms(row_squares(mine, waves * 64 * N, lane), a);  // (zeros behind the row's end)
             __syncthreads();
         }
-        auto codes = [&](int64_t c, int i) {
-            if (cols == 0 || c >= ra.kp) return;  // (whole groups)
+        auto codes = [&](uint32_t c, int i) {
+            if (cols == 0 || c >= static_cast<uint32_t>(ra.kp)) return;  // (whole groups)
             if (h) store_row<VEC>(h, c, cols, v[i]);
             float w[kElems], code[kElems];
             if (norm) floats_as<VEC>(wr[i], a.weight_dtype, w);
-            const float s = group_codes(v[i], w, norm, inv, a.group, c - c % a.group < cols, code);
+            const float s = group_codes(v[i], w, norm, inv, a.group, (c & -static_cast<uint32_t>(a.group)) < cols, code);
             *reinterpret_cast<uint2*>(a.q + r * ra.kp + c) = make_uint2(four_codes(code), four_codes(code + 4));
-            if (c % a.group == 0) a.scales[r * (ra.kp / a.group) + c / a.group] = s;
+            if ((c & (a.group - 1)) == 0) a.scales[r * (ra.kp >> ra.shift) + (c >> ra.shift)] = s;
             if (a.values) {
 #pragma unroll
                 for (int e = 0; e < kElems; ++e) code[e] *= s;
@@ -108,11 +134,14 @@ __global__ __launch_bounds__(1024) void rows_kernel(RowsArgs ra) {
         };
         if constexpr (CH > 0) {
 #pragma unroll
-            for (int i = 0; i < CH; ++i) codes(tid * kElems + i * step, i);
+            for (int i = 0; i < CH; ++i) {
+                codes(tid * kElems + i * step, i);
+                __builtin_amdgcn_sched_barrier(0);  // (runs interleaved took more registers than there are)
+            }
         } else {
             for (int i = 0; i < passes; ++i) {
-                const int64_t c = tid * kElems + static_cast<int64_t>(i) * step;
-                fetch(c, 0);
+                const uint32_t c = tid * kElems + i * step;
+                fetch(r, c, 0);
                 if (norm) load_raw_as<VEC>(a.weight, c, a.cols, a.weight_dtype, wr[0]);
                 hidden(0);
                 codes(c, 0);
@@ -132,62 +161,57 @@ struct PackArgs {
 
 __device__ __forceinline__ float quarter_max(float v) { return xmax16(xmax32(v)); }  // over lanes l, l ^ 16, l ^ 32, l ^ 48
 
-// One wave per tile: lane 16 j + r holds row r's columns 32 b + 8 j .. + 7 of the tile, b < 4.
+// One workgroup per tile, wave b its columns 32 b .. + 31: lane 16 j + r holds row r's eight from 8 j.  What a group wider than
+// 32 columns and a byte's two halves need of other waves goes through LDS.  (One wave per tile, with a true
+// quotient a value, took as long for large matrices, at the rate of a copy, but 6.8 us for 2049 x 387 against 4.1.)
 template <class T, int G, bool VEC>
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
-    const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
+    __shared__ float tops[4][16];
+    __shared__ uint2 halves[4][64];
+    const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4, b = threadIdx.x >> 6;
     const int kb = (a.k + kTileCols - 1) / kTileCols;
-    const int64_t tiles = static_cast<int64_t>((a.n + kTileRows - 1) / kTileRows) * kb;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (t >= tiles) return;
-    const int64_t row = t / kb * kTileRows + r;
-    const int c0 = static_cast<int>(t % kb) * kTileCols + 8 * j;
-    const T* src = static_cast<const T*>(a.w) + row * a.stride;
-    Raw<kElems> raw[4];
-    float v[4][kElems];
+    const int64_t t = blockIdx.x, row = t / kb * kTileRows + r;
+    Raw<kElems> raw;
+    float v[kElems];
+    load_raw<VEC>(static_cast<const T*>(a.w) + row * a.stride, t % kb * kTileCols + 32 * b + 8 * j, row < a.n ? a.k : 0, raw);
+    floats<VEC, T>(raw, v);
+    // the larger of max w / 7 and -min w / 8, or infinity where a value is not finite
+    float mx = -INFINITY, mn = -INFINITY, bad = 0.0f;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) load_raw<VEC>(src, c0 + 32 * b, row < a.n ? a.k : 0, raw[b]);
-#pragma unroll
-    for (int b = 0; b < 4; ++b) floats<VEC, T>(raw[b], v[b]);
-    uint32_t out[4] = {0, 0, 0, 0};
-    constexpr int B = G / 32, NG = 4 / B;
-    uint16_t sc[NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        float mx = -INFINITY, mn = -INFINITY, bad = 0.0f;
-#pragma unroll
-        for (int b = g * B; b < (g + 1) * B; ++b)
-#pragma unroll
-            for (int i = 0; i < kElems; ++i) {
-                mx = fmaxf(mx, v[b][i]);
-                mn = fmaxf(mn, -v[b][i]);
-                bad = __builtin_fmaf(v[b][i], 0.0f, bad);
-            }
-        mx = quarter_max(mx);
-        mn = quarter_max(mn);
-        const float wrong = quarter_max(bad == 0.0f ? 0.0f : 1.0f);
-        const __bf16 sb = static_cast<__bf16>(fmaxf(mx / 7.0f, mn / 8.0f));
-        float s = static_cast<float>(sb);
-        if (wrong != 0.0f || !(fabsf(s) <= 3.402823466e38f)) s = __uint_as_float(0x7fc00000u);
-        sc[g] = static_cast<uint16_t>(__float_as_uint(s) >> 16);
-#pragma unroll
-        for (int b = g * B; b < (g + 1) * B; ++b)
-#pragma unroll
-            for (int i = 0; i < kElems; ++i) {
-                // The quotient is rounded to FP32, which could put it on a half; the remainder, exact
-                // (q s has 12 bits and is next to v), tells.  A remainder of s / 2 is a half indeed, and q even.
-                float q = rintf(v[b][i] / s);
-                const float rem = __builtin_fmaf(-q, s, v[b][i]);
-                if (2.0f * fabsf(rem) > s) q += copysignf(1.0f, rem);
-                q = fminf(fmaxf(q, -8.0f), 7.0f);
-                const int code = s > 0.0f ? static_cast<int>(q) : 0;
-                out[2 * (b >> 1) + (i >> 2)] |= (static_cast<uint32_t>(code) & 15u) << (8 * (i & 3) + 4 * (b & 1));
-            }
+    for (int i = 0; i < kElems; ++i) {
+        mx = fmaxf(mx, v[i]);
+        mn = fmaxf(mn, -v[i]);
+        bad = __builtin_fmaf(v[i], 0.0f, bad);
     }
-    *reinterpret_cast<u32x4*>(a.packed + t * kTileBytes + lane * 16) = u32x4{out[0], out[1], out[2], out[3]};
-    if (j == 0) {
+    float top = quarter_max(bad == 0.0f ? fmaxf(mx / 7.0f, mn / 8.0f) : INFINITY);
+    if constexpr (G > 32) {
+        if (j == 0) tops[b][r] = top;
+        __syncthreads();
+        top = fmaxf(tops[b][r], tops[b ^ 1][r]);
+        if constexpr (G > 64) top = fmaxf(top, fmaxf(tops[b ^ 2][r], tops[b ^ 3][r]));
+    }
+    float s = static_cast<float>(static_cast<__bf16>(top));
+    if (!(fabsf(s) <= 3.402823466e38f)) s = __uint_as_float(0x7fc00000u);
+    // Codes: v / s by the reciprocal, at most one off; the remainder (exact by fma: q s has 12 bits and is next to v)
+    // says whether, and finds the halves, which go to the even one.  Tiny numbers are scaled by 2^64 first.
+    const float up = s < 1e-30f ? 18446744073709551616.0f : 1.0f, su = s * up, inv = 1.0f / su;
+    uint32_t out[2] = {0, 0};
 #pragma unroll
-        for (int g = 0; g < NG; ++g) a.scales[(t * kTileRows + r) * NG + g] = sc[g];
+    for (int i = 0; i < kElems; ++i) {
+        const float vu = v[i] * up;
+        float q = rintf(vu * inv);
+        const float rem = __builtin_fmaf(-q, su, vu), two = 2.0f * fabsf(rem);
+        if (two > su || (two == su && (static_cast<int>(q) & 1))) q += copysignf(1.0f, rem);
+        q = fminf(fmaxf(q, -8.0f), 7.0f);
+        out[i >> 2] |= (s > 0.0f ? static_cast<uint32_t>(static_cast<int>(q)) & 15u : 0u) << (8 * (i & 3));
+    }
+    halves[b][lane] = make_uint2(out[0], out[1]);
+    constexpr int NG = 128 / G;
+    if (j == 0 && b % (G / 32) == 0) a.scales[(t * kTileRows + r) * NG + b / (G / 32)] = static_cast<uint16_t>(__float_as_uint(s) >> 16);
+    __syncthreads();
+    if (b < 2) {
+        const uint2 lo = halves[2 * b][lane], hi = halves[2 * b + 1][lane];
+        *reinterpret_cast<uint2*>(a.packed + t * kTileBytes + lane * 16 + 8 * b) = make_uint2(lo.x | hi.x << 4, lo.y | hi.y << 4);
     }
 }
 
@@ -199,18 +223,22 @@ struct UnpackArgs {
     int64_t stride;
 };
 
+// One wave per tile.  FP32 rows go through LDS, so that half a wave writes 512 bytes in a row past the caches (85 -> 54 us for
+// 16384 x 5120; 74 through them).
 template <class T, int G, bool VEC>
 __global__ __launch_bounds__(256) void unpack_kernel(UnpackArgs a) {
-    const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
+    constexpr bool STAGED = VEC && sizeof(T) == 4;
+    constexpr int kRow = kTileCols + 4;
+    __shared__ __align__(16) float staged[STAGED ? 4 * kTileRows * kRow : 4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, j = lane >> 4;
     const int kb = (a.k + kTileCols - 1) / kTileCols;
     const int64_t tiles = static_cast<int64_t>((a.n + kTileRows - 1) / kTileRows) * kb;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * 4 + wave;
     if (t >= tiles) return;
-    const int64_t row = t / kb * kTileRows + r;
-    if (row >= a.n) return;
+    const int64_t row0 = t / kb * kTileRows, row = row0 + r;
     const u32x4 w = *reinterpret_cast<const u32x4*>(a.packed + t * kTileBytes + lane * 16);
-    T* dst = static_cast<T*>(a.out) + row * a.stride;
-    const int c0 = static_cast<int>(t % kb) * kTileCols + 8 * j;
+    const int c0 = static_cast<int>(t % kb) * kTileCols;
+    float* mine = staged + wave * kTileRows * kRow;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
         const float s = bf16_to_f32(a.scales[(t * kTileRows + r) * (128 / G) + 32 * b / G]);
@@ -220,7 +248,24 @@ __global__ __launch_bounds__(256) void unpack_kernel(UnpackArgs a) {
             const int shift = 8 * (i & 3) + 4 * (b & 1);
             v[i] = static_cast<float>(static_cast<int32_t>(w[2 * (b >> 1) + (i >> 2)] << (28 - shift)) >> 28) * s;
         }
-        store_row<VEC>(dst, c0 + 32 * b, a.k, v);
+        if constexpr (STAGED) {
+            float4* at = reinterpret_cast<float4*>(mine + r * kRow + 32 * b + 8 * j);
+            at[0] = make_float4(v[0], v[1], v[2], v[3]);
+            at[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            store_row<VEC>(static_cast<T*>(a.out) + row * a.stride, c0 + 32 * b + 8 * j, row < a.n ? a.k : 0, v);
+        }
+    }
+    if constexpr (STAGED) {
+        wave_sync();
+        const int col = 4 * (lane & 31);
+#pragma unroll
+        for (int i = 0; i < kTileRows / 2; ++i) {
+            const int rr = 2 * i + (lane >> 5);
+            const f32x4 v = *reinterpret_cast<const f32x4*>(mine + rr * kRow + col);
+            if (row0 + rr < a.n && c0 + col < a.k)
+                __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + (row0 + rr) * a.stride + c0 + col));
+        }
     }
 }
 
@@ -326,12 +371,6 @@ __device__ __forceinline__ void tile_best(float2* best, int tile, int tiles, flo
     if (lane == 0 && tile < tiles) best[tile] = make_float2(v, i);
 }
 
-// Orders a wave's LDS accesses before and after it.
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // Up to four tokens: bound by the weights' bytes and, for small matrices, by latency.  A workgroup owns NT
 // tile rows (16 weight rows each) and all columns; its waves take every W-th tile of 128 columns, U at a
 // time, with all loads of a turn requested before their first use, and add their sums through LDS in
@@ -346,7 +385,8 @@ constexpr int kFewRow = kTileCols + 8;  // four rows' pieces lie in different ba
 template <int G, int NT, int U, bool FUSED>
 __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
     const ProductArgs& a = fa.p;
-    if (fa.active && !*fa.active) return;
+    // (asked for first, waited for once the first loads are under way)
+    const uint32_t active = fa.active ? *fa.active : 1u;
     constexpr int NG = 128 / G;
     // codes by blocks of 128 columns: [block][token][136 bytes], and scales [block][token][NG]; all blocks
     // of one token (FUSED), or those of a wave's turn
@@ -430,6 +470,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
 #pragma unroll
         for (int i = 0; i < KEEP; ++i)
             if (tid + i * T < quads) request(tid + i * T, x0[i], w0[i]);
+        if (!active) return;
 #pragma unroll
         for (int i = 0; i < KEEP; ++i) convert(x0[i], w0[i], v0[i], g0[i]);
         if (r.weight) {
@@ -454,6 +495,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
         }
         __syncthreads();
     }
+    if (!active) return;
     // the wave's own places for a turn's codes and scales, which whole cache lines bring there
     const int own = wave * U * kFewTokens, piece = lane & 7, token_c = min(lane >> 3, rows - 1);
     const int8_t* xg = FUSED ? nullptr : a.q + static_cast<int64_t>(token_c) * kb * kTileCols + 16 * piece;
@@ -835,20 +877,24 @@ int pad_cols(int64_t k) { return static_cast<int>((k + kTileCols - 1) / kTileCol
 }  // namespace
 
 constexpr int kFewRows = 512;
+constexpr int kRowGroups = 1024;  // workgroups that are resident together, about: each goes through several rows
 
 hipError_t launch_rows(const NormArgs& a, hipStream_t s) {
     if (a.rows == 0) return hipSuccess;
     const bool vec = a.cols % kElems == 0 && rows_aligned(a.x, a.x_stride, a.dtype) && rows_aligned(a.residual, a.residual_stride, a.dtype) &&
                      rows_aligned(a.h_out, a.h_stride, a.dtype) && rows_aligned(a.values, a.values_stride, a.dtype) &&
                      rows_aligned(a.weight, 0, a.dtype);
-    // Waves a row takes with one run of 512 columns each.  Few rows: as many (up to 16), for their latency; many rows: two or
-    // four runs a wave, whose loads are under way at once.
+    // Waves a row takes with one run of 512 columns each.  Few rows: as many (up to 16), for their latency.  Many
+    // rows: one, two or four waves and up to four runs each, whose loads are under way at once; and teams that
+    // fill workgroups of four waves, or a multiple: of five waves a SIMD got two in every workgroup, and 8192 x
+    // 5120 took 118 us instead of 81.
     const int kp = pad_cols(a.cols), all = (kp + 511) / 512;
-    int ch = all <= 16 && a.rows <= kFewRows ? 1 : all <= 1 ? 1 : all <= 32 ? 2 : all <= 64 ? 4 : 0;
-    const int waves = ch ? (all + ch - 1) / ch : kLongThreads / 64;
+    const bool few = all <= 16 && a.rows <= kFewRows;
+    const int waves = few ? all : all == 1 ? 1 : all <= 4 ? (all + 1) / 2 : all <= 16 ? 4 : all <= 32 ? 8 : 16;
+    const int ch = few ? 1 : all <= 64 ? (all + waves - 1) / waves : 0;
     const int teams = waves >= 4 ? 1 : 4 / waves;
-    const RowsArgs ra{a, kp, waves};
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((a.rows + teams - 1) / teams, 1 << 20))), block(64 * waves * teams);
+    const RowsArgs ra{a, kp, waves, a.group == 32 ? 5 : a.group == 64 ? 6 : 7};
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((a.rows + teams - 1) / teams, kRowGroups))), block(64 * waves * teams);
     return by_type(a.dtype, [&](auto t) {
         using T = decltype(t);
         return by_bool(vec, [&](auto v) {
@@ -856,6 +902,7 @@ hipError_t launch_rows(const NormArgs& a, hipStream_t s) {
                 constexpr bool V = decltype(v)::value, R = decltype(res)::value;
                 if (ch == 1) hipLaunchKernelGGL((rows_kernel<T, 1, V, R>), grid, block, 0, s, ra);
                 else if (ch == 2) hipLaunchKernelGGL((rows_kernel<T, 2, V, R>), grid, block, 0, s, ra);
+                else if (ch == 3) hipLaunchKernelGGL((rows_kernel<T, 3, V, R>), grid, block, 0, s, ra);
                 else if (ch == 4) hipLaunchKernelGGL((rows_kernel<T, 4, V, R>), grid, block, 0, s, ra);
                 else hipLaunchKernelGGL((rows_kernel<T, 0, V, R>), grid, block, 0, s, ra);
                 return hipGetLastError();
@@ -987,7 +1034,7 @@ hipError_t launch_pack(const void* w, int64_t stride, int dtype, int n, int k, i
     const PackArgs a{w, stride, n, k, static_cast<uint8_t*>(packed), static_cast<uint16_t*>(scales)};
     const bool vec = k % kElems == 0 && rows_aligned(w, stride, dtype);
     const int64_t tiles = static_cast<int64_t>((n + kTileRows - 1) / kTileRows) * (pad_cols(k) / kTileCols);
-    const dim3 grid(static_cast<unsigned>((tiles + 3) / 4));
+    const dim3 grid(static_cast<unsigned>(tiles));
     return by_type(dtype, [&](auto t) {
         return by_group(group, [&](auto g) {
             return by_bool(vec, [&](auto v) {

@@ -129,7 +129,7 @@ struct Raw {
     uint32_t w[E];  // four bytes an element, or (VEC, two-byte types) two elements a word
 };
 template <bool VEC, class T, int E>
-__device__ __forceinline__ void load_raw(const T* row, int64_t c, int64_t cols, Raw<E>& out) {
+__device__ __forceinline__ void load_raw(const T* row, uint32_t c, uint32_t cols, Raw<E>& out) {
 #pragma unroll
     for (int i = 0; i < E; ++i) out.w[i] = 0;
     if constexpr (VEC) {
@@ -164,7 +164,7 @@ __device__ __forceinline__ void floats(const Raw<E>& in, float (&out)[E]) {
     }
 }
 template <bool VEC, class T>
-__device__ __forceinline__ void store_row(T* row, int64_t c, int64_t cols, const float (&in)[kElems]) {
+__device__ __forceinline__ void store_row(T* row, uint32_t c, uint32_t cols, const float (&in)[kElems]) {
     if constexpr (VEC) {
         constexpr int P = 16 / sizeof(T);
         if (c < cols) {
@@ -234,7 +234,14 @@ __device__ __forceinline__ float group_codes(const float (&v)[E], const float (&
         }
         if (off > 0.4999f) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) q[i] = static_cast<float>(rint(exact(i) * inv / static_cast<double>(s)));
+            for (int i = 0; i < E; ++i) {
+                // |y| against the half between the two codes next to it, (k + 1 / 2) s, exact in 64 bits
+                const double y = fabs(exact(i) * inv);
+                const float k = floorf(fabsf(p[i] * cf) - 0.4f);
+                const double half = (static_cast<double>(k) + 0.5) * static_cast<double>(s);
+                const bool odd = static_cast<int>(k) & 1;
+                if (fabsf(fabsf(p[i] * cf) - k - 0.5f) < 0.4f) q[i] = copysignf(y > half || (y == half && odd) ? k + 1.0f : k, p[i]);
+            }
         }
         return s;
     }
