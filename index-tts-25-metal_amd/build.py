@@ -98,7 +98,7 @@ def build_ops_module() -> Path:
         f"-I{INCLUDE}", f"-isystem{base / 'include'}", f"-isystem{base / 'include/torch/csrc/api/include'}",
         f"-isystem{Path(HIPCC).parent.parent / 'include'}", f"-isystem{sysconfig.get_paths()['include']}",
         str(CSRC / "ops_torch.cpp"),
-        f"-L{PKG}", "-litts_gpt", f"-L{base / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
+        f"-L{PKG}", "-litts_gpt", f"-L{base / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python",
         "-Wl,-rpath,$ORIGIN",
         "-o", str(tmp),
     ])

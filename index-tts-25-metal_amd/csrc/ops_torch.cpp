@@ -10,6 +10,7 @@
 #include <string>
 
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -147,6 +148,7 @@ public:
         if (!t) return;
         if (!t->is_cuda()) no("tensors have to be on the GPU");
         if (t->device() != first_.device()) no("tensors on ", first_.device().str(), " and ", t->device().str());
+        if (t->is_neg()) no("a negated view: resolve_neg() it first");
         if (t->requires_grad() && c10::GradMode::is_enabled())
             no("these operators have no gradients: detach the tensors, or call under torch.no_grad()");
     }
@@ -179,7 +181,7 @@ void done(int status) {
 }
 void* at_of(const Tensor* t) { return t ? t->data_ptr() : nullptr; }
 
-Tensor make(at::IntArrayRef sizes, const Tensor& like_, at::ScalarType type) { return at::empty(sizes, like_.options().dtype(type)); }
+Tensor make(at::IntArrayRef sizes, const Tensor& like_, at::ScalarType type) { return at::detail::empty_cuda(sizes, type, like_.device(), std::nullopt); }
 
 PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
 

@@ -52,9 +52,15 @@ struct FewArgs {
     const uint32_t* token;   // or null: x is row *token of a matrix (launch_fused)
     float* h_out;            // or null: receives x's row in F32 (launch_fused)
     float2* best;            // or null: per 16 weight rows the largest sum of row 0 and its index
+    const float* parts;      // launch_merged: attention over splits of 64 cache rows, [split][k / 128 heads][128], weighted sums
+    const float* part_ml;    //   [split][heads][2]: the largest score and the sum of exp(score - largest); both hold 64 splits
+    const uint32_t* cached;  //   cache rows before this step's: cached / 64 + 1 splits count
     bool vec;                // set by launch_fused
 };
 hipError_t launch_few(const FewArgs& a, hipStream_t s);
+// launch_fused for a decode step's attention output, whose splits it merges: x[128 h + d] = sum over splits of w_s parts[s][h][d] /
+// sum of w_s ml[s][h][1], w_s = exp(ml[s][h][0] - their largest).  k a multiple of 128, group 128.
+hipError_t launch_merged(const FewArgs& a, hipStream_t s);
 bool linear_is_fused(int64_t rows, int64_t n, int64_t k);
 hipError_t launch_fused(const FewArgs& a, hipStream_t s);
 // Norm (or quantisation) and product: fused, or through rows.q and rows.scales.

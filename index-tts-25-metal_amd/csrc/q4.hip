@@ -381,9 +381,13 @@ __device__ __forceinline__ void tile_best(float2* best, int tile, int tiles, flo
 // turn's weights already under way: one launch instead of two, 6.4 -> 4.2 us for one row x 4096 x 1024.
 // (Four rows by every workgroup took longer than a launch of their own: 14.8 us against 8.4 for 4 x 10240 x 1280.)
 constexpr int kFewWaves = 8, kFewTokens = 4, kFusedCols = 16384;
+// Where the tokens come from: codes; a float row; or a decode step's attention, in parts over splits of the cache.
+enum : int { kFromCodes = 0, kFromRow = 1, kFromParts = 2 };
+constexpr uint32_t kSplitRows = 64;  // cache rows a split
 constexpr int kFewRow = kTileCols + 8;  // four rows' pieces lie in different banks
-template <int G, int NT, int U, bool FUSED>
+template <int G, int NT, int U, int FROM>
 __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
+    constexpr bool FUSED = FROM != kFromCodes;
     const ProductArgs& a = fa.p;
     // (asked for first, waited for once the first loads are under way)
     const uint32_t active = fa.active ? *fa.active : 1u;
@@ -394,7 +398,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
     __shared__ __align__(16) uint8_t codes[kBlocks * kFewRow];
     __shared__ float scales[kBlocks * NG];
     __shared__ float sums[kFewWaves * NT * 64];
-    __shared__ double squares[FUSED ? kFusedCols / kElems : 1];
+    __shared__ double squares[FROM == kFromRow ? kFusedCols / kElems : 1];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, quarter = lane >> 4;
     const int W = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kb = (a.k + kTileCols - 1) / kTileCols, tiles = (a.n + kTileRows - 1) / kTileRows;
@@ -417,8 +421,63 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
             }
         }
     };
-    if constexpr (FUSED) {
-        weights(blockIdx.x, wave);
+    if constexpr (FUSED) weights(blockIdx.x, wave);
+    if constexpr (FROM == kFromParts) {
+        // Four columns a thread, half a wave a head.  Its lanes hold the splits' largest scores and sums, two each, and
+        // form the splits' weights at once; the first splits' values are asked for before their number is known.
+        constexpr int TURN = 8;
+        const uint32_t cached = *fa.cached;
+        for (int p = tid; p < kb * 32; p += blockDim.x) {
+            const int head = p >> 5, l = p & 31;
+            auto v_at = [&](int s) { return *reinterpret_cast<const float4*>(fa.parts + (static_cast<size_t>(s) * kb + head) * kTileCols + l * 4); };
+            const float2* ml = reinterpret_cast<const float2*>(fa.part_ml) + head;
+            float2 a0 = ml[l * kb], a1 = ml[(l + 32) * kb];
+            float4 v[TURN];
+#pragma unroll
+            for (int s = 0; s < TURN; ++s) v[s] = v_at(s);
+            if (!active) return;
+            const int splits = static_cast<int>(cached / kSplitRows) + 1;
+            if (l >= splits) a0 = make_float2(-INFINITY, 0.0f);
+            if (l + 32 >= splits) a1 = make_float2(-INFINITY, 0.0f);
+            auto over_half = [](float x, auto op) {
+                x = op(x, lane_of<1>(x));
+                x = op(x, lane_of<2>(x));
+                x = op(x, lane_of<4>(x));
+                x = op(x, lane_of<8>(x));
+                return op(x, lane_of<16>(x));
+            };
+            const float top = over_half(fmaxf(a0.x, a1.x), [](float x, float y) { return fmaxf(x, y); });
+            const float w0 = expf(a0.x - top), w1 = expf(a1.x - top);
+            const float den = over_half(__builtin_fmaf(w1, a1.y, w0 * a0.y), [](float x, float y) { return x + y; });
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}, none[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+            for (int s0 = 0; s0 < splits; s0 += TURN) {
+                float4 x[TURN];
+#pragma unroll
+                for (int s = 0; s < TURN; ++s) x[s] = v[s];
+                if (s0 + TURN < splits) {
+#pragma unroll
+                    for (int s = 0; s < TURN; ++s) v[s] = v_at(min(s0 + TURN + s, splits - 1));
+                }
+#pragma unroll
+                for (int s = 0; s < TURN; ++s) {
+                    if (s0 + s >= splits) break;
+                    const float w = __shfl(s0 < 32 ? w0 : w1, (lane & 32) | ((s0 + s) & 31));
+                    sum[0] = __builtin_fmaf(w, x[s].x, sum[0]);
+                    sum[1] = __builtin_fmaf(w, x[s].y, sum[1]);
+                    sum[2] = __builtin_fmaf(w, x[s].z, sum[2]);
+                    sum[3] = __builtin_fmaf(w, x[s].w, sum[3]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] /= den;
+            float code[4];
+            const float s = group_codes(sum, none, false, 1.0, G, true, code);
+            *reinterpret_cast<uint32_t*>(codes + head * kFewRow + (p & 31) * 4) = four_codes(code);
+            if (p * 4 % G == 0) scales[p * 4 / G] = s;
+        }
+        __syncthreads();
+    }
+    if constexpr (FROM == kFromRow) {
         const NormArgs& r = fa.rows;
         const int T = blockDim.x, quads = kb * 32;
         const int64_t first = fa.token ? *fa.token : 0;
@@ -925,24 +984,24 @@ int turn_tiles(int each) {
     return u;
 }
 
-template <int G, int NT, int U, bool FUSED>
+template <int G, int NT, int U, int FROM>
 hipError_t launch_few(const FewArgs& a, int waves, hipStream_t s) {
     const int tiles = (a.p.n + kTileRows - 1) / kTileRows;
-    hipLaunchKernelGGL((few_kernel<G, NT, U, FUSED>), dim3((tiles + NT - 1) / NT), dim3(64 * waves), 0, s, a);
+    hipLaunchKernelGGL((few_kernel<G, NT, U, FROM>), dim3((tiles + NT - 1) / NT), dim3(64 * waves), 0, s, a);
     return hipGetLastError();
 }
-template <int G, bool FUSED>
+template <int G, int FROM>
 hipError_t few_rows(const FewArgs& a, hipStream_t s) {
     const int kb = pad_cols(a.p.k) / kTileCols, waves = std::min(kb, kFewWaves), each = (kb + waves - 1) / waves;
-    if constexpr (!FUSED) {
-        if (a.p.n >= kFewWide) return each == 1 ? launch_few<G, 4, 1, FUSED>(a, waves, s) : launch_few<G, 4, 2, FUSED>(a, waves, s);
+    if constexpr (FROM == kFromCodes) {
+        if (a.p.n >= kFewWide) return each == 1 ? launch_few<G, 4, 1, FROM>(a, waves, s) : launch_few<G, 4, 2, FROM>(a, waves, s);
     }
     switch (turn_tiles(each)) {
-        case 1: return launch_few<G, 1, 1, FUSED>(a, waves, s);
-        case 2: return launch_few<G, 1, 2, FUSED>(a, waves, s);
-        case 3: return launch_few<G, 1, 3, FUSED>(a, waves, s);
-        case 4: return launch_few<G, 1, 4, FUSED>(a, waves, s);
-        default: return launch_few<G, 1, 5, FUSED>(a, waves, s);
+        case 1: return launch_few<G, 1, 1, FROM>(a, waves, s);
+        case 2: return launch_few<G, 1, 2, FROM>(a, waves, s);
+        case 3: return launch_few<G, 1, 3, FROM>(a, waves, s);
+        case 4: return launch_few<G, 1, 4, FROM>(a, waves, s);
+        default: return launch_few<G, 1, 5, FROM>(a, waves, s);
     }
 }
 template <int G, int NT, int U>
@@ -971,7 +1030,7 @@ hipError_t launch_tiles(const ProductArgs& a, hipStream_t s) {
 }
 template <int G>
 hipError_t product(const ProductArgs& a, hipStream_t s) {
-    if (a.rows <= kFewTokens) return few_rows<G, false>(FewArgs{a}, s);
+    if (a.rows <= kFewTokens) return few_rows<G, kFromCodes>(FewArgs{a}, s);
 #ifdef VAR
     const int var = std::getenv("VAR") ? std::atoi(std::getenv("VAR")) : 0;
     switch (var) {
@@ -1010,14 +1069,16 @@ hipError_t launch_product(const ProductArgs& given, hipStream_t s) {
 bool linear_is_fused(int64_t rows, int64_t n, int64_t k) { return rows == 1 && n <= 1024 * kTileRows && k <= kFusedCols; }
 
 hipError_t launch_few(const FewArgs& a, hipStream_t s) {
-    return by_group(a.p.group, [&](auto g) { return few_rows<decltype(g)::value, false>(a, s); });
+    return by_group(a.p.group, [&](auto g) { return few_rows<decltype(g)::value, kFromCodes>(a, s); });
 }
 
 hipError_t launch_fused(const FewArgs& given, hipStream_t s) {
     FewArgs a = given;
     a.vec = a.p.k % kElems == 0 && rows_aligned(a.rows.x, a.rows.x_stride, a.rows.dtype) && rows_aligned(a.rows.weight, 0, a.rows.dtype);
-    return by_group(a.p.group, [&](auto g) { return few_rows<decltype(g)::value, true>(a, s); });
+    return by_group(a.p.group, [&](auto g) { return few_rows<decltype(g)::value, kFromRow>(a, s); });
 }
+
+hipError_t launch_merged(const FewArgs& a, hipStream_t s) { return few_rows<128, kFromParts>(a, s); }
 
 hipError_t launch_linear(const ProductArgs& product, const NormArgs& rows, hipStream_t s) {
     if (product.rows == 0) return hipSuccess;
@@ -1080,6 +1141,9 @@ int ops_guarded(F&& f) {
     } catch (const std::exception& e) {
         g_ops_error = e.what();
         return ITTS_ERUNTIME;
+    } catch (...) {
+        g_ops_error = "Unknown failure";
+        return ITTS_ERUNTIME;
     }
 }
 
@@ -1093,8 +1157,30 @@ bool type_ok(int32_t t) { return t == ITTS_T_F32 || t == ITTS_T_BF16 || t == ITT
 bool group_ok(int32_t g) { return g == 32 || g == 64 || g == 128; }
 // Sizes up to these keep every index that the kernels form in 32 bits where they use 32, and every grid in range.
 constexpr int64_t kMaxRows = int64_t(1) << 30, kMaxN = int64_t(1) << 26, kMaxK = int64_t(1) << 20;
+constexpr int64_t kMaxResults = int64_t(1) << 36;
 bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 bool aligned_for(const void* p, int32_t dtype) { return aligned(p, dtype == ITTS_T_F32 ? 4 : 2); }
+
+// A matrix in memory: rows of `width` bytes, `step` bytes apart.
+struct Span {
+    const void* at;
+    int64_t rows, width, step;
+    Span(const void* p, int64_t r, int64_t cols, int64_t stride, int32_t dtype) : at(p), rows(r), width(cols * static_cast<int64_t>(type_size(dtype))), step(width) {
+        if (r <= 1) return;
+        need(!p || stride <= (int64_t(1) << 56) / (4 * r), "Row stride out of range");
+        step = p ? stride * static_cast<int64_t>(type_size(dtype)) : width;
+    }
+    bool same(const Span& o) const { return at == o.at && step == o.step; }
+    // Whether the two share a byte (or, with different steps, might): columns of one wider matrix do not.
+    bool meets(const Span& o) const {
+        if (!at || !o.at) return false;
+        const int64_t a = static_cast<int64_t>(reinterpret_cast<uintptr_t>(at)), b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(o.at));
+        if (a + (rows - 1) * step + width <= b || b + (o.rows - 1) * o.step + o.width <= a) return false;
+        if (step != o.step || step < width || step < o.width) return true;
+        const int64_t d = ((b - a) % step + step) % step;  // where o's rows begin in this one's
+        return d < width || d + o.width > step;
+    }
+};
 
 void check_rows(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int32_t group, const void* values,
                 int64_t values_stride, const int8_t* q, const float* scales) {
@@ -1106,6 +1192,7 @@ void check_rows(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, in
     need(x && q && scales, "Missing tensor");
     need(x_stride >= 0 && (!values || rows == 1 || values_stride >= cols), "Row stride out of range");
     need(aligned_for(x, dtype) && aligned_for(values, dtype) && aligned(q, 16) && aligned(scales, 4), "Misaligned tensor");
+    need(!Span(values, rows, cols, values_stride, dtype).meets(Span(x, rows, cols, x_stride, dtype)), "Output overlaps an input");
 }
 
 void check_weight(const void* packed, const void* scales, int64_t n, int64_t k, int32_t group) {
@@ -1127,6 +1214,10 @@ ProductArgs product_args(int64_t rows, const void* packed, const void* scales, i
         need(out, "Missing tensor");
         need(residual_stride >= 0 && (rows == 1 || out_stride >= (swiglu ? n / 2 : n)), "Row stride out of range");
         need(aligned_for(out, dtype) && aligned_for(residual, dtype) && aligned(bias, 4), "Misaligned tensor");
+        need(rows * n <= kMaxResults, "Too many results");
+        const int64_t cols = swiglu ? n / 2 : n;
+        const Span os(out, rows, cols, out_stride, dtype), rs(residual, rows, cols, residual_stride, dtype);
+        need(os.same(rs) || !os.meets(rs), "Output overlaps an input");
     }
     ProductArgs p{};
     p.rows = static_cast<int>(rows);
@@ -1163,6 +1254,9 @@ int itts_rmsnorm_q8(const void* x, int64_t x_stride, const void* residual, int64
         need(weight, "Missing tensor");
         need(residual_stride >= 0 && (!h_out || rows == 1 || h_stride >= cols), "Row stride out of range");
         need(aligned_for(residual, dtype) && aligned_for(h_out, dtype) && aligned_for(weight, weight_dtype), "Misaligned tensor");
+        const Span xs(x, rows, cols, x_stride, dtype), rs(residual, rows, cols, residual_stride, dtype), hs(h_out, rows, cols, h_stride, dtype),
+            vs(values, rows, cols, values_stride, dtype);
+        need((hs.same(xs) || !hs.meets(xs)) && (hs.same(rs) || !hs.meets(rs)) && !vs.meets(rs) && !vs.meets(hs), "Output overlaps an input");
         NormArgs a{x, x_stride, residual, residual_stride, weight, weight_dtype, dtype, rows, cols, eps, group, h_out, h_stride, values,
                    values_stride, q, scales};
         launched(launch_rows(a, static_cast<hipStream_t>(stream)));
@@ -1244,6 +1338,8 @@ int itts_q4_linear(const void* x, int64_t x_stride, int32_t x_dtype, int64_t row
         need(x, "Missing tensor");
         need(x_stride >= 0, "Row stride out of range");
         need(aligned_for(x, x_dtype) && (!norm_weight || aligned_for(norm_weight, weight_dtype)), "Misaligned tensor");
+        // (workgroups that norm the row for themselves read x while others write out)
+        need(!Span(out, rows, p.swiglu ? n / 2 : n, out_stride, dtype).meets(Span(x, rows, k, x_stride, x_dtype)), "Output overlaps an input");
         const size_t bytes = itts_q4_linear_workspace(rows, n, k, group);
         need(bytes == 0 || (workspace && workspace_bytes >= bytes), "Workspace too small");
         need(aligned(workspace, 256), "Misaligned workspace");

@@ -1029,14 +1029,20 @@ struct Engine {
             QAttnArgs aa{qkv.p, K(l), Vc(l), N(l) + kNormQ, N(l) + kNormK, inv_freq.p, part_acc.p, part_ml.p, att.p, st.p};
             hipLaunchKernelGGL(q_attn_kernel, dim3(kAttnGrid), dim3(256), 0, s, aa);
             QWEN_CHECK(hipGetLastError());
-            hipLaunchKernelGGL(q_attn_merge_kernel, dim3(kQH), dim3(kHd), 0, s, aa);
-            QWEN_CHECK(hipGetLastError());
             if (q4_layers) {
-                q4_step(q4[l].o, att.p, false, nullptr, h.p, h.p, false);
+                // the splits are merged by the output projection's workgroups, each for itself
+                q4::FewArgs m{q4_product(q4[l].o, 1, h.p, h.p, false)};
+                m.active = &st.p->active;
+                m.cached = &st.p->cached;
+                m.parts = part_acc.p;
+                m.part_ml = part_ml.p;
+                QWEN_CHECK(q4::launch_merged(m, stream));
                 q4_step(q4[l].gu, h.p, false, N(l) + kNormPost, ff.p, nullptr, true);
                 q4_step(q4[l].d, ff.p, false, nullptr, h.p, h.p, false);
                 continue;
             }
+            hipLaunchKernelGGL(q_attn_merge_kernel, dim3(kQH), dim3(kHd), 0, s, aa);
+            QWEN_CHECK(hipGetLastError());
             QGemvArgs o{};
             o.st = st.p;
             o.w = w + kOffO;

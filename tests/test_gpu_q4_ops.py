@@ -308,6 +308,29 @@ def test_linear_may_add_to_its_own_rows(ops):
         assert torch.equal(ops.q4_linear(x, w, residual=h, out=h), want)
 
 
+def test_outputs_over_inputs(itts, ops):
+    """A product over its own rows is refused; columns of one wider matrix are apart."""
+    r = rng(31)
+    w, _, _ = weight_of(ops, r, 256, 256, 128)
+    for rows in (1, 3, 40):
+        x = tensor(r.standard_normal((rows, 256)))
+        with pytest.raises(itts.InvalidArgument, match="overlaps"):
+            ops.q4_linear(x, w, out=x)
+        wide = torch.zeros(rows, 600, device="cuda")
+        wide[:, 300:556] = x
+        got = ops.q4_linear(wide[:, 300:556], w, out=wide[:, 20:276])
+        assert torch.equal(got, ops.q4_linear(x, w)) and torch.equal(wide[:, 300:556], x)
+        with pytest.raises(itts.InvalidArgument, match="overlaps"):
+            ops.rmsnorm_q8(x, torch.ones(256, device="cuda"), residual=x.clone(), values=x)
+    with pytest.raises(itts.InvalidArgument, match="negated"):
+        ops.q8_quantize(torch._neg_view(torch.zeros(2, 64, device="cuda")))
+    a, b = torch.ones(2, 64, device="cuda", requires_grad=True), torch.ones(64, device="cuda")
+    with pytest.raises(itts.InvalidArgument, match="no gradients"):
+        ops.rmsnorm_q8(a, b)
+    with torch.no_grad():
+        ops.rmsnorm_q8(a, b)
+
+
 # ------------------------------------------------------------------ a layer's run of them
 def layer(ops, x, r_in, ws, nws, dtype):
     a = ops.rmsnorm_q8(x, nws[0], 1e-6, residual=r_in)

@@ -106,6 +106,23 @@ def test_prefill_and_steps_stay_within_the_rounding(itts, qw, rounded, n_prompt)
         assert np.all(np.isfinite(g)) and e <= BAR, (i, e)
 
 
+@pytest.mark.parametrize("n_prompt", [510, 2046])
+def test_steps_merge_many_splits(itts, oracle, n_prompt):
+    """One layer, caches of 8 and 9, and of 32 and 33 splits of 64 rows, which the output projection merges."""
+    w = itts.make_synthetic_qwen_weights(layers=1, seed=23)
+    d = itts.QwenDecoder(w, layers=1, weight_bits=4, head_bits=32)
+    orc = oracle.OracleQwen({k: four_bits(v) if k.endswith(MATRICES) else v for k, v in w.items()}, layers=1)
+    p, bar = ids_of(n_prompt, n_prompt + 5), 2 * 0.0091 * np.sqrt(5)
+    print(f"{n_prompt} ids, one layer", flush=True)
+    d.prefill(p[:n_prompt])
+    orc.prefill(p[:n_prompt])
+    for i in range(5):
+        e = rel_err(d.step(p[n_prompt + i]), orc.step(p[n_prompt + i]))
+        print(f"row {n_prompt + i}: {e:.4f} (bar {bar:.4f})", flush=True)
+        assert e <= bar
+    d.close()
+
+
 def test_steps_continue_a_prefill(dec):
     """A prefill of n ids and steps, and one of n + 3: the same cache up to the 8-bit rounding's moves (as the bar)."""
     p = ids_of(5, 70)

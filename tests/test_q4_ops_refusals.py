@@ -151,6 +151,16 @@ def test_the_c_abi_refuses(itts, ops):
                {"work": C.c_void_p((1 << 20) + 16)}, {"out": None}, {"x": C.c_void_p((1 << 20) + 2)}):
         assert linear(**kw) == -1, kw
 
+    # outputs over inputs
+    off = lambda n: C.c_void_p((1 << 20) + n)  # noqa: E731
+    for kw in ({"v": at, "vs": 64}, {"h": off(4), "hs": 64}, {"h": at, "hs": 65}, {"res": off(128), "rs": 64, "h": at, "hs": 64},
+               {"v": off(256), "vs": 64}, {"x": at, "xs": 128, "h": off(252), "hs": 128}):
+        assert norm(**kw) == -1 and b"overlaps" in lib.itts_ops_last_error(), kw
+    for kw in ({"out": off(100), "os": 128}, {"rows": 1, "out": off(100), "os": 128}):
+        assert linear(**kw) == -1 and b"overlaps" in lib.itts_ops_last_error(), kw
+    assert matmul(res=off(4), rs=32) == -1 and b"overlaps" in lib.itts_ops_last_error()
+    assert matmul(rows=1 << 19, n=1 << 20, os=1 << 20) == -1 and b"Too many" in lib.itts_ops_last_error()
+
     def pack(w=at, ws=128, t=0, n=32, k=128, g=128, p=at, s=at):
         return lib.itts_q4_pack(w, ws, t, n, k, g, p, s, None)
 
