@@ -710,8 +710,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void batch_kernel(ProductArgs a) {
 }
 
 // More than 16 tokens: bound by the scaling.  Every group's 32-bit sums take a conversion, the product of
-// the two scales and a multiply-add a value in the vector units, which at groups of 128 is about what the matrix units need for the
-// group.  A workgroup owns 32 WM MT tokens x 32 WN NT weight rows.  WM x WN waves share a tile of codes staged through
+// the two scales and a multiply-add a value in the vector units, and those add to the matrix instructions' time rather than
+// hide beside it: at 2048 x 10240 x 5120 in groups of 128 a block of 32 x 32 and a group costs about 300 cycles of the former
+// and 130 of the latter, and runs in 480 (161 us).  The outer product of scales as a matrix instruction of its own took 171 us,
+// the last block of a turn scaled beside the next turn's products 163 (and 174 became 247 in blocks of 128 x 128).  A workgroup owns 32 WM MT tokens x 32 WN NT weight rows.  WM x WN waves share a tile of codes staged through
 // LDS; weights go from memory to registers, in the order of the instruction's operand; the next turn's loads
 // are under way while this one's are multiplied.  WK such groups of waves take every WK-th tile of columns and
 // add their sums through LDS in order.
@@ -1031,18 +1033,6 @@ hipError_t launch_tiles(const ProductArgs& a, hipStream_t s) {
 template <int G>
 hipError_t product(const ProductArgs& a, hipStream_t s) {
     if (a.rows <= kFewTokens) return few_rows<G, kFromCodes>(FewArgs{a}, s);
-#ifdef VAR
-    const int var = std::getenv("VAR") ? std::atoi(std::getenv("VAR")) : 0;
-    switch (var) {
-        case 1: return launch_batch<G, 1, 1>(a, std::min(8, (a.k + 127) / 128), s);
-        case 2: return launch_batch<G, 1, 2>(a, std::min(8, (a.k + 127) / 128), s);
-        case 3: return launch_batch<G, 1, 5>(a, std::min(8, (a.k + 127) / 128), s);
-        case 4: return launch_batch<G, 2, 1>(a, std::min(8, (a.k + 127) / 128), s);
-        case 5: return launch_batch<G, 4, 1>(a, std::min(8, (a.k + 127) / 128), s);
-        case 6: return launch_batch<G, 2, 5>(a, std::min(8, (a.k + 127) / 128), s);
-        case 7: return launch_batch<G, 2, 3>(a, std::min(8, (a.k + 127) / 128), s);
-    }
-#endif
     if (a.rows <= 16) return batch_rows<G>(a, s);
     // Workgroups of 64 x 128 (one wave 64 x 32: the fewest LDS and memory reads a product) where two a CU come of
     // them; else of 64 x 64, nearly as many; else smaller blocks whose waves share the columns, for the latency of

@@ -71,7 +71,7 @@ def test_one_id_is_the_operators_one_after_the_other(itts, ops, qw, dec, head_bi
                 m = lambda *n: torch.cat([t[p + x + ".weight"] for x in n])  # noqa: E731
                 qkv = ops.q4_linear(h, ops.q4_pack(m("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj"), GROUP),
                                     norm_weight=t[p + "input_layernorm.weight"])
-                att = qkv[:, 3072:].view(8, 1, 128).expand(8, 2, 128).reshape(1, 2048)
+                att = qkv[:, -1024:].view(8, 1, 128).expand(8, 2, 128).reshape(1, 2048)
                 h = ops.q4_linear(att, ops.q4_pack(m("self_attn.o_proj"), GROUP), residual=h)
                 gu = torch.stack([t[p + "mlp.gate_proj.weight"], t[p + "mlp.up_proj.weight"]], 1).view(-1, 1024)
                 ff = ops.q4_linear(h, ops.q4_pack(gu, GROUP), norm_weight=t[p + "post_attention_layernorm.weight"], swiglu=True)
