@@ -11,9 +11,10 @@
  * into a graph and may run at once from several threads and streams, as long as their outputs
  * and workspaces are apart.  Matrices are row-major with unit column stride; strides are row
  * strides in elements, at least the columns for outputs.  An output may be one of the call's inputs where
- * this says so; otherwise they do not overlap (columns of one wider matrix do not).  A call with no
+ * this says so; otherwise outputs and workspace overlap neither inputs nor each other (columns of one wider
+ * matrix do not), which the calls check.  A call with no
  * rows does nothing.  Up to 2^20 columns k, 2^26 weight rows n, 2^30 rows (products: 1048560, and
- * rows * n up to 2^36).
+ * rows * n up to 2^36; packing and unpacking: 2^33 packed bytes).
  *
  * Status codes are those of itts_gpt.h: ITTS_EINVAL for arguments that the checks refuse (nothing
  * is enqueued), ITTS_ERUNTIME for a failed launch.  itts_ops_last_error() has the message of the

@@ -12,6 +12,7 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -181,6 +182,13 @@ void done(int status) {
 }
 void* at_of(const Tensor* t) { return t ? t->data_ptr() : nullptr; }
 
+// A given output: autograd has to see that its values change.
+const Tensor& written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    else if (!c10::InferenceMode::is_enabled()) no("an output made in inference mode, outside of it");
+    return t;
+}
+
 Tensor make(at::IntArrayRef sizes, const Tensor& like_, at::ScalarType type) { return at::detail::empty_cuda(sizes, type, like_.device(), std::nullopt); }
 
 PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
@@ -199,7 +207,7 @@ Codes codes(const Tensor& x, int64_t rows, int64_t cols, int64_t group, const Te
                    !scales->is_contiguous()))
         no("scales: contiguous float32 [", rows, ", ", kp / group, "] is wanted");
     on();
-    return {q ? *q : make({rows, kp}, x, at::kChar), scales ? *scales : make({rows, kp / group}, x, at::kFloat)};
+    return {q ? written(*q) : make({rows, kp}, x, at::kChar), scales ? written(*scales) : make({rows, kp / group}, x, at::kFloat)};
 }
 
 // (x, weight or None, eps, residual, group, h, q, scales, values) -> (h, q, scales, values)
@@ -228,9 +236,9 @@ PyObject* rows_to_codes(PyObject* const* a, bool norm) {
         on.enter();
     });
     Tensor h, v;
-    if (h_in) h = *h_in;
+    if (h_in) h = written(*h_in);
     else if (residual) h = make({m.rows, m.cols}, x, x.scalar_type());
-    if (v_in) v = *v_in;
+    if (v_in) v = written(*v_in);
     else if (values) v = make({m.rows, m.cols}, x, x.scalar_type());
     void* const hp = h.defined() ? h.data_ptr() : nullptr;
     void* const vp = v.defined() ? v.data_ptr() : nullptr;
@@ -291,7 +299,7 @@ PyObject* unpack(PyObject* const* a) {
     on.also(w.scales);
     on.also(given);
     on.enter();
-    const Tensor out = given ? *given : make({w.n, w.k}, *w.packed, type_of(kind));
+    const Tensor out = given ? written(*given) : make({w.n, w.k}, *w.packed, type_of(kind));
     done(itts_q4_unpack(w.packed->data_ptr(), w.scales->data_ptr(), w.n, w.k, static_cast<int32_t>(w.group), kind, out.data_ptr(), os, on.stream()));
     return wrap(out);
 }
@@ -323,7 +331,7 @@ struct Product {
     void on(const On& o, const Weight& w) const {
         for (const Tensor* t : {w.packed, w.scales, bias, residual, given}) o.also(t);
     }
-    Tensor out(int64_t rows, const Tensor& x) const { return given ? *given : make({rows, cols}, x, type_of(kind)); }
+    Tensor out(int64_t rows, const Tensor& x) const { return given ? written(*given) : make({rows, cols}, x, type_of(kind)); }
     const float* bias_at() const { return static_cast<const float*>(at_of(bias)); }
     uint32_t flags() const { return swiglu ? ITTS_Q4_SWIGLU : 0u; }
 };

@@ -1,5 +1,6 @@
 // Operators on 4-bit weights and 8-bit activations (include/itts_ops.h): kernels, launchers and C ABI.
 #include <algorithm>
+#include <initializer_list>
 #include <stdexcept>
 #include <string>
 
@@ -1148,6 +1149,8 @@ bool group_ok(int32_t g) { return g == 32 || g == 64 || g == 128; }
 // Sizes up to these keep every index that the kernels form in 32 bits where they use 32, and every grid in range.
 constexpr int64_t kMaxRows = int64_t(1) << 30, kMaxN = int64_t(1) << 26, kMaxK = int64_t(1) << 20;
 constexpr int64_t kMaxResults = int64_t(1) << 36;
+// A workgroup of 256 a tile: fewer than 2^32 threads, the most that a launch takes.
+constexpr size_t kMaxPacked = size_t(kTileBytes) << 23;
 bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 bool aligned_for(const void* p, int32_t dtype) { return aligned(p, dtype == ITTS_T_F32 ? 4 : 2); }
 
@@ -1160,15 +1163,21 @@ struct Span {
         need(!p || stride <= (int64_t(1) << 56) / (4 * r), "Row stride out of range");
         step = p ? stride * static_cast<int64_t>(type_size(dtype)) : width;
     }
+    Span(const void* p, size_t bytes) : at(p), rows(1), width(static_cast<int64_t>(bytes)), step(width) {}
     bool same(const Span& o) const { return at == o.at && step == o.step; }
     // Whether the two share a byte (or, with different steps, might): columns of one wider matrix do not.
     bool meets(const Span& o) const {
         if (!at || !o.at) return false;
         const int64_t a = static_cast<int64_t>(reinterpret_cast<uintptr_t>(at)), b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(o.at));
         if (a + (rows - 1) * step + width <= b || b + (o.rows - 1) * o.step + o.width <= a) return false;
-        if (step != o.step || step < width || step < o.width) return true;
-        const int64_t d = ((b - a) % step + step) % step;  // where o's rows begin in this one's
-        return d < width || d + o.width > step;
+        if (rows == 1 && o.rows == 1) return true;
+        const int64_t s = rows > 1 ? step : o.step;
+        if ((o.rows > 1 && o.step != s) || s < width || s < o.width) return true;
+        const int64_t d = ((b - a) % s + s) % s;  // where o's rows begin in this one's
+        return d < width || d + o.width > s;
+    }
+    void apart(std::initializer_list<Span> others) const {
+        for (const Span& o : others) need(!meets(o), "Output overlaps an input or another output");
     }
 };
 
@@ -1182,7 +1191,12 @@ void check_rows(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, in
     need(x && q && scales, "Missing tensor");
     need(x_stride >= 0 && (!values || rows == 1 || values_stride >= cols), "Row stride out of range");
     need(aligned_for(x, dtype) && aligned_for(values, dtype) && aligned(q, 16) && aligned(scales, 4), "Misaligned tensor");
-    need(!Span(values, rows, cols, values_stride, dtype).meets(Span(x, rows, cols, x_stride, dtype)), "Output overlaps an input");
+    const int64_t kp = pad_cols(cols);
+    const Span xs(x, rows, cols, x_stride, dtype), vs(values, rows, cols, values_stride, dtype), qs(q, static_cast<size_t>(rows * kp)),
+        ss(scales, static_cast<size_t>(rows * (kp / group)) * sizeof(float));
+    vs.apart({xs, qs, ss});
+    qs.apart({xs, ss});
+    ss.apart({xs});
 }
 
 void check_weight(const void* packed, const void* scales, int64_t n, int64_t k, int32_t group) {
@@ -1191,6 +1205,10 @@ void check_weight(const void* packed, const void* scales, int64_t n, int64_t k, 
     need(packed && scales, "Missing tensor");
     need(aligned(packed, 16) && aligned(scales, 16), "Misaligned tensor");
 }
+
+Span packed_span(const void* packed, int64_t n, int64_t k) { return {packed, itts_q4_packed_bytes(n, k)}; }
+Span scales_span(const void* scales, int64_t n, int64_t k, int32_t group) { return {scales, itts_q4_scale_count(n, k, group) * 2}; }
+Span out_span(const ProductArgs& p) { return {p.out, p.rows, p.swiglu ? p.n / 2 : p.n, p.out_stride, p.dtype}; }
 
 ProductArgs product_args(int64_t rows, const void* packed, const void* scales, int64_t n, int64_t k, int32_t group, const float* bias,
                          const void* residual, int64_t residual_stride, uint32_t flags, int32_t dtype, void* out, int64_t out_stride) {
@@ -1208,6 +1226,7 @@ ProductArgs product_args(int64_t rows, const void* packed, const void* scales, i
         const int64_t cols = swiglu ? n / 2 : n;
         const Span os(out, rows, cols, out_stride, dtype), rs(residual, rows, cols, residual_stride, dtype);
         need(os.same(rs) || !os.meets(rs), "Output overlaps an input");
+        os.apart({packed_span(packed, n, k), scales_span(scales, n, k, group), Span(bias, static_cast<size_t>(n) * sizeof(float))});
     }
     ProductArgs p{};
     p.rows = static_cast<int>(rows);
@@ -1246,7 +1265,13 @@ int itts_rmsnorm_q8(const void* x, int64_t x_stride, const void* residual, int64
         need(aligned_for(residual, dtype) && aligned_for(h_out, dtype) && aligned_for(weight, weight_dtype), "Misaligned tensor");
         const Span xs(x, rows, cols, x_stride, dtype), rs(residual, rows, cols, residual_stride, dtype), hs(h_out, rows, cols, h_stride, dtype),
             vs(values, rows, cols, values_stride, dtype);
-        need((hs.same(xs) || !hs.meets(xs)) && (hs.same(rs) || !hs.meets(rs)) && !vs.meets(rs) && !vs.meets(hs), "Output overlaps an input");
+        const Span ws(weight, static_cast<size_t>(cols) * type_size(weight_dtype)), qs(q, static_cast<size_t>(rows * pad_cols(cols))),
+            ss(scales, static_cast<size_t>(rows * (pad_cols(cols) / group)) * sizeof(float));
+        need((hs.same(xs) || !hs.meets(xs)) && (hs.same(rs) || !hs.meets(rs)), "Output overlaps an input");
+        hs.apart({vs, qs, ss, ws});
+        vs.apart({rs, ws});
+        qs.apart({rs, ws});
+        ss.apart({rs, ws});
         NormArgs a{x, x_stride, residual, residual_stride, weight, weight_dtype, dtype, rows, cols, eps, group, h_out, h_stride, values,
                    values_stride, q, scales};
         launched(launch_rows(a, static_cast<hipStream_t>(stream)));
@@ -1280,6 +1305,10 @@ int itts_q4_pack(const void* w, int64_t w_stride, int32_t dtype, int64_t n, int6
         need(w, "Missing tensor");
         need(w_stride >= 0, "Row stride out of range");
         need(aligned_for(w, dtype), "Misaligned tensor");
+        need(itts_q4_packed_bytes(n, k) <= kMaxPacked, "Weight too large");
+        const Span ps = packed_span(packed, n, k), ss = scales_span(scales, n, k, group), ws(w, n, k, w_stride, dtype);
+        ps.apart({ss, ws});
+        ss.apart({ws});
         launched(launch_pack(w, w_stride, dtype, static_cast<int>(n), static_cast<int>(k), group, packed, scales, static_cast<hipStream_t>(stream)));
     });
 }
@@ -1292,6 +1321,8 @@ int itts_q4_unpack(const void* packed, const void* scales, int64_t n, int64_t k,
         need(out, "Missing tensor");
         need(n == 1 || out_stride >= k, "Row stride out of range");
         need(aligned_for(out, dtype), "Misaligned tensor");
+        need(itts_q4_packed_bytes(n, k) <= kMaxPacked, "Weight too large");
+        Span(out, n, k, out_stride, dtype).apart({packed_span(packed, n, k), scales_span(scales, n, k, group)});
         launched(launch_unpack(packed, scales, static_cast<int>(n), static_cast<int>(k), group, dtype, out, out_stride, static_cast<hipStream_t>(stream)));
     });
 }
@@ -1306,6 +1337,8 @@ int itts_q4_matmul(const int8_t* q, const float* qscales, int64_t rows, const vo
         need(aligned(q, 16) && aligned(qscales, 4), "Misaligned tensor");
         p.q = q;
         p.qscales = qscales;
+        const int64_t kp = pad_cols(k);
+        out_span(p).apart({Span(q, static_cast<size_t>(rows * kp)), Span(qscales, static_cast<size_t>(rows * (kp / group)) * sizeof(float))});
         launched(launch_product(p, static_cast<hipStream_t>(stream)));
     });
 }
@@ -1329,10 +1362,14 @@ int itts_q4_linear(const void* x, int64_t x_stride, int32_t x_dtype, int64_t row
         need(x_stride >= 0, "Row stride out of range");
         need(aligned_for(x, x_dtype) && (!norm_weight || aligned_for(norm_weight, weight_dtype)), "Misaligned tensor");
         // (workgroups that norm the row for themselves read x while others write out)
-        need(!Span(out, rows, p.swiglu ? n / 2 : n, out_stride, dtype).meets(Span(x, rows, k, x_stride, x_dtype)), "Output overlaps an input");
+        const Span xs(x, rows, k, x_stride, x_dtype), ns(norm_weight, static_cast<size_t>(k) * type_size(weight_dtype)), os = out_span(p);
+        os.apart({xs, ns});
         const size_t bytes = itts_q4_linear_workspace(rows, n, k, group);
         need(bytes == 0 || (workspace && workspace_bytes >= bytes), "Workspace too small");
         need(aligned(workspace, 256), "Misaligned workspace");
+        if (bytes)
+            Span(workspace, bytes).apart({xs, ns, os, packed_span(packed, n, k), scales_span(scales, n, k, group), Span(bias, static_cast<size_t>(n) * sizeof(float)),
+                                          Span(residual, rows, p.swiglu ? n / 2 : n, residual_stride, dtype)});
         int8_t* q = static_cast<int8_t*>(workspace);
         float* qs = bytes ? reinterpret_cast<float*>(q + codes_bytes(rows, k)) : nullptr;
         const NormArgs r{x, x_stride, nullptr, 0, norm_weight, weight_dtype, x_dtype, rows, k, eps, group, nullptr, 0, nullptr, 0, q, qs};

@@ -331,6 +331,55 @@ def test_outputs_over_inputs(itts, ops):
         ops.rmsnorm_q8(a, b)
 
 
+def test_outputs_over_weights_and_scales(itts, ops):
+    """The same for the tensors beside the rows; a scale matrix as wide as the product is one of them."""
+    w, _, _ = weight_of(ops, rng(32), 2, 256, 128)
+    norm, bias = torch.ones(256, device="cuda"), torch.ones(2, device="cuda")
+    eight = ops.q8_quantize(tensor(rng(33).standard_normal((1, 256))), 128)
+    with pytest.raises(itts.InvalidArgument, match="overlaps"):
+        ops.q4_matmul(eight.q, eight.scales, w, out=eight.scales)
+    with pytest.raises(itts.InvalidArgument, match="overlaps"):
+        ops.q4_matmul(eight.q, eight.scales, w, bias=bias, out=bias[None])
+    with pytest.raises(itts.InvalidArgument, match="overlaps"):
+        ops.q4_linear(torch.ones(1, 256, device="cuda"), w, norm_weight=norm, out=norm[None, :2])
+    with pytest.raises(itts.InvalidArgument, match="overlaps"):
+        ops.rmsnorm_q8(torch.ones(1, 256, device="cuda"), norm, h=norm[None])
+
+
+def test_autograd_sees_given_outputs_change(itts, ops):
+    """A tensor that a backward pass keeps may not be written unseen; one of inference mode only in it."""
+    w, _, _ = weight_of(ops, rng(34), 256, 256, 128)
+    x, norm = tensor(rng(35).standard_normal((3, 256))), torch.ones(256, device="cuda")
+    eight = ops.rmsnorm_q8(x, norm, values=True)
+    outs = {
+        "q4_matmul": lambda o: ops.q4_matmul(eight.q, eight.scales, w, out=o),
+        "q4_linear": lambda o: ops.q4_linear(x, w, out=o),
+        "h": lambda o: ops.rmsnorm_q8(x, norm, h=o),
+        "values": lambda o: ops.q8_quantize(x, values=o),
+    }
+    for name, call in outs.items():
+        kept, leaf = torch.ones(3, 256, device="cuda"), torch.ones(3, 256, device="cuda", requires_grad=True)
+        loss = (leaf * kept).sum()
+        with torch.no_grad():
+            call(kept)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        with torch.inference_mode():
+            mine = torch.ones(3, 256, device="cuda")
+            call(mine)
+        assert torch.equal(mine, kept), name
+        with pytest.raises(itts.InvalidArgument, match="inference mode"):
+            call(mine)
+    for t in (eight.q, eight.scales, x):
+        before = t._version
+        ops.rmsnorm_q8(x, norm, h=x, q=eight.q, scales=eight.scales)
+        assert t._version == before + 1
+    full = ops.q4_unpack(w)
+    before = full._version
+    ops.q4_unpack(w, out=full)
+    assert full._version == before + 1
+
+
 # ------------------------------------------------------------------ a layer's run of them
 def layer(ops, x, r_in, ws, nws, dtype):
     a = ops.rmsnorm_q8(x, nws[0], 1e-6, residual=r_in)

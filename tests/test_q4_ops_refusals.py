@@ -119,60 +119,95 @@ def test_two_hip_runtimes_are_refused():
         assert (p.returncode == 0) == one and (one or not fine), (order, p.stderr[-500:])
 
 
-def test_the_c_abi_refuses(itts, ops):
-    """Addresses that are never read: every call here ends in its checks, with a message."""
-    lib, at = library(itts), C.c_void_p(1 << 20)
+def place(i, off=0):
+    """The i-th of some addresses 2^24 bytes apart (no buffer below is larger), and off bytes behind it."""
+    return C.c_void_p(((i + 1) << 24) + off)
 
-    def norm(x=at, xs=64, res=None, rs=0, w=at, wt=0, t=0, rows=2, cols=64, eps=1e-6, g=64, h=None, hs=0, v=None, vs=0, q=at, s=at):
+
+def calls(itts):
+    """The C ABI's calls with arguments that would be accepted, each in a place of its own."""
+    lib = library(itts)
+
+    def norm(x=place(0), xs=64, res=None, rs=64, w=place(1), wt=0, t=0, rows=2, cols=64, eps=1e-6, g=64, h=None, hs=64, v=None, vs=64, q=place(2), s=place(3)):
         return lib.itts_rmsnorm_q8(x, xs, res, rs, w, wt, t, rows, cols, eps, g, h, hs, v, vs, q, s, None)
 
-    assert norm(rows=0) == 0
-    for kw in ({"x": None}, {"w": None}, {"q": None}, {"s": None}, {"xs": -1}, {"t": 3}, {"t": -1}, {"wt": 1}, {"t": 1, "wt": 2}, {"rows": -1},
-               {"rows": 1 << 40}, {"cols": 0}, {"cols": 1 << 40}, {"eps": -1.0}, {"eps": float("nan")}, {"g": 0}, {"g": 16}, {"h": at, "hs": 63},
-               {"v": at, "vs": 63}, {"res": at, "rs": -1}, {"q": C.c_void_p((1 << 20) + 8)}, {"x": C.c_void_p((1 << 20) + 1)},
-               {"s": C.c_void_p((1 << 20) + 2)}, {"w": C.c_void_p((1 << 20) + 2)}):
-        assert norm(**kw) == -1 and lib.itts_ops_last_error(), kw
-
-    def matmul(q=at, qs=at, rows=2, p=at, s=at, n=32, k=128, g=128, bias=None, res=None, rs=0, flags=0, t=0, out=at, os=32):
+    def matmul(q=place(0), qs=place(1), rows=2, p=place(2), s=place(3), n=32, k=128, g=128, bias=None, res=None, rs=32, flags=0, t=0, out=place(4), os=32):
         return lib.itts_q4_matmul(q, qs, rows, p, s, n, k, g, bias, res, rs, flags, t, out, os, None)
 
-    assert matmul(rows=0) == 0
-    for kw in ({"q": None}, {"qs": None}, {"p": None}, {"s": None}, {"out": None}, {"n": 0}, {"n": 1 << 40}, {"k": 0}, {"k": 1 << 40}, {"g": 1},
-               {"flags": 2}, {"t": 7}, {"os": 31}, {"n": 33, "flags": 1, "os": 40}, {"rows": -1}, {"rows": 1 << 40}, {"res": at, "rs": -2},
-               {"q": C.c_void_p((1 << 20) + 4)}, {"p": C.c_void_p((1 << 20) + 4)}, {"out": C.c_void_p((1 << 20) + 2)}, {"bias": C.c_void_p((1 << 20) + 1)}):
-        assert matmul(**kw) == -1, kw
+    def linear(x=place(0), xs=128, xt=0, rows=200, nw=None, wt=0, eps=0.0, p=place(1), s=place(2), n=32, k=128, g=128, bias=None, res=None, rs=32, flags=0, t=0,
+               out=place(3), os=32, work=place(4), bytes_=1 << 20):
+        return lib.itts_q4_linear(x, xs, xt, rows, nw, wt, eps, p, s, n, k, g, bias, res, rs, flags, t, out, os, work, bytes_, None)
 
-    def linear(x=at, xs=128, xt=0, rows=200, nw=None, wt=0, eps=0.0, p=at, s=at, n=32, k=128, g=128, flags=0, t=0, out=at, os=32, work=at, bytes_=1 << 30):
-        return lib.itts_q4_linear(x, xs, xt, rows, nw, wt, eps, p, s, n, k, g, None, None, 0, flags, t, out, os, work, bytes_, None)
+    def pack(w=place(0), ws=128, t=0, n=32, k=128, g=128, p=place(1), s=place(2)):
+        return lib.itts_q4_pack(w, ws, t, n, k, g, p, s, None)
+
+    def unpack(p=place(0), s=place(1), n=32, k=128, g=128, t=0, out=place(2), os=128):
+        return lib.itts_q4_unpack(p, s, n, k, g, t, out, os, None)
+
+    return lib, norm, matmul, linear, pack, unpack
+
+
+def test_the_c_abi_refuses(itts, ops):
+    """Addresses that are never read: every call here ends in its checks, with a message."""
+    lib, norm, matmul, linear, pack, unpack = calls(itts)
+
+    def no(fn, *cases, message=b""):
+        for kw in cases:
+            assert fn(**kw) == -1 and lib.itts_ops_last_error() and message in lib.itts_ops_last_error(), kw
+            assert b"overlaps" not in lib.itts_ops_last_error(), kw
+
+    assert norm(rows=0) == 0
+    no(norm, {"x": None}, {"w": None}, {"q": None}, {"s": None}, message=b"Missing")
+    no(norm, {"xs": -1}, {"h": place(5), "hs": 63}, {"v": place(5), "vs": 63}, {"res": place(5), "rs": -1}, message=b"stride")
+    no(norm, {"t": 3}, {"t": -1}, {"wt": 1}, {"t": 1, "wt": 2}, {"rows": -1}, {"rows": 1 << 40}, {"cols": 0}, {"cols": 1 << 40}, {"eps": -1.0},
+       {"eps": float("nan")}, {"g": 0}, {"g": 16})
+    no(norm, {"q": place(2, 8)}, {"x": place(0, 1)}, {"s": place(3, 2)}, {"w": place(1, 2)}, message=b"Misaligned")
+
+    assert matmul(rows=0) == 0
+    no(matmul, {"q": None}, {"qs": None}, {"p": None}, {"s": None}, {"out": None}, message=b"Missing")
+    no(matmul, {"n": 0}, {"n": 1 << 40}, {"k": 0}, {"k": 1 << 40}, {"g": 1}, {"flags": 2}, {"t": 7}, {"n": 33, "flags": 1, "os": 40}, {"rows": -1}, {"rows": 1 << 40})
+    no(matmul, {"os": 31}, {"res": place(5), "rs": -2}, message=b"stride")
+    no(matmul, {"q": place(0, 4)}, {"p": place(2, 4)}, {"out": place(4, 2)}, {"bias": place(5, 1)}, message=b"Misaligned")
+    no(matmul, {"rows": 1 << 19, "n": 1 << 20, "os": 1 << 20}, message=b"Too many")
 
     need = lib.itts_q4_linear_workspace(200, 32, 128, 128)
     assert need >= 200 * 132 and linear(rows=0) == 0
-    for kw in ({"x": None}, {"xs": -1}, {"xt": 5}, {"nw": at, "wt": 1}, {"nw": at, "eps": -1.0}, {"work": None}, {"bytes_": need - 1},
-               {"work": C.c_void_p((1 << 20) + 16)}, {"out": None}, {"x": C.c_void_p((1 << 20) + 2)}):
-        assert linear(**kw) == -1, kw
+    no(linear, {"x": None}, {"out": None}, message=b"Missing")
+    no(linear, {"xs": -1}, {"xt": 5}, {"nw": place(5), "wt": 1}, {"nw": place(5), "eps": -1.0})
+    no(linear, {"work": None}, {"bytes_": need - 1}, {"work": place(4, 16)}, message=b"orkspace")
+    no(linear, {"x": place(0, 2)}, message=b"Misaligned")
 
-    # outputs over inputs
-    off = lambda n: C.c_void_p((1 << 20) + n)  # noqa: E731
-    for kw in ({"v": at, "vs": 64}, {"h": off(4), "hs": 64}, {"h": at, "hs": 65}, {"res": off(128), "rs": 64, "h": at, "hs": 64},
-               {"v": off(256), "vs": 64}, {"x": at, "xs": 128, "h": off(252), "hs": 128}):
-        assert norm(**kw) == -1 and b"overlaps" in lib.itts_ops_last_error(), kw
-    for kw in ({"out": off(100), "os": 128}, {"rows": 1, "out": off(100), "os": 128}):
-        assert linear(**kw) == -1 and b"overlaps" in lib.itts_ops_last_error(), kw
-    assert matmul(res=off(4), rs=32) == -1 and b"overlaps" in lib.itts_ops_last_error()
-    assert matmul(rows=1 << 19, n=1 << 20, os=1 << 20) == -1 and b"Too many" in lib.itts_ops_last_error()
-
-    def pack(w=at, ws=128, t=0, n=32, k=128, g=128, p=at, s=at):
-        return lib.itts_q4_pack(w, ws, t, n, k, g, p, s, None)
-
-    def unpack(p=at, s=at, n=32, k=128, g=128, t=0, out=at, os=128):
-        return lib.itts_q4_unpack(p, s, n, k, g, t, out, os, None)
-
-    for kw in ({"w": None}, {"ws": -1}, {"t": 9}, {"n": 0}, {"k": 0}, {"g": 2}, {"p": None}, {"s": None}, {"p": C.c_void_p((1 << 20) + 1)}):
-        assert pack(**kw) == -1, kw
-    for kw in ({"out": None}, {"os": 127}, {"t": 9}, {"n": 0}, {"k": 0}, {"g": 2}, {"p": None}, {"s": None}):
-        assert unpack(**kw) == -1, kw
+    no(pack, {"w": None}, {"ws": -1}, {"t": 9}, {"n": 0}, {"k": 0}, {"g": 2}, {"p": None}, {"s": None}, {"p": place(1, 1)})
+    no(unpack, {"out": None}, {"os": 127}, {"t": 9}, {"n": 0}, {"k": 0}, {"g": 2}, {"p": None}, {"s": None})
+    # a workgroup a tile: no more tiles than a launch can have
+    no(pack, {"n": 1 << 26, "k": 257, "ws": 0}, message=b"too large")
+    no(unpack, {"n": 1 << 26, "k": 257, "os": 257}, message=b"too large")
     assert lib.itts_q4_packed_bytes(17, 129) == 4 * 1024 and lib.itts_q4_packed_bytes(0, 5) == 0 and lib.itts_q4_packed_bytes(1 << 40, 5) == 0
     assert lib.itts_q4_scale_count(17, 129, 32) == 4 * 64 and lib.itts_q4_scale_count(17, 129, 31) == 0
+
+
+def test_outputs_over_inputs_and_each_other(itts, ops):
+    """Workgroups write an output while others still read the inputs: no byte may belong to both."""
+    lib, norm, matmul, linear, pack, unpack = calls(itts)
+
+    def overlaps(fn, *cases):
+        for kw in cases:
+            assert fn(**kw) == -1 and b"overlaps" in lib.itts_ops_last_error(), (kw, lib.itts_ops_last_error())
+
+    x, w, q, s, other = place(0), place(1), place(2), place(3), place(5)
+    overlaps(norm, {"v": x}, {"h": place(0, 4)}, {"h": x, "hs": 65}, {"res": place(0, 128), "h": x}, {"v": place(0, 256)},
+             {"xs": 128, "h": place(0, 252), "hs": 128})
+    overlaps(norm, {"h": w}, {"v": w}, {"v": other, "h": other}, {"h": q}, {"v": q}, {"h": s}, {"v": s}, {"h": place(3, -508)}, {"q": x}, {"q": place(0, 496)},
+             {"q": w}, {"res": other, "q": other}, {"s": x}, {"s": w}, {"res": other, "s": other}, {"s": place(2, 124)}, {"rows": 1, "h": w})
+    p, bias = place(2), {"bias": other}
+    overlaps(matmul, {"out": place(0)}, {"out": place(0, 252)}, {"out": place(1)}, {"out": place(1, -252)}, {"out": p}, {"out": place(2, 2048 - 4)}, {"out": s},
+             {"out": place(3, 64 - 4)}, {**bias, "out": other}, {**bias, "out": other, "rows": 1}, {"out": place(5, 124), **bias}, {"res": place(4, 4)})
+    overlaps(linear, {"out": place(0, 100), "os": 128}, {"rows": 1, "out": place(0, 100), "os": 128}, {"nw": place(3)}, {"rows": 1, "nw": place(3)},
+             {"out": place(1)}, {"out": place(2)}, {"out": other, **bias})
+    overlaps(linear, {"work": place(0)}, {"work": place(1)}, {"work": place(2)}, {"work": place(3)}, {"work": other, **bias}, {"work": other, "res": other},
+             {"work": other, "nw": other})
+    overlaps(pack, {"p": place(0)}, {"s": place(0)}, {"s": place(1)}, {"s": place(1, 2032)}, {"p": place(0, 4096)})
+    overlaps(unpack, {"out": place(0)}, {"out": place(1)}, {"out": place(0, 2044)}, {"out": place(1, -512), "n": 2})
 
 
 def test_weight_bits(itts):
