@@ -18,10 +18,10 @@ __device__ __forceinline__ void load_raw_as(const void* row, uint32_t c, uint32_
     else load_raw<VEC>(static_cast<const _Float16*>(row), c, cols, out);
 }
 template <bool VEC, int E>
-__device__ __forceinline__ void floats_as(const Raw<E>& in, int dtype, float (&out)[E]) {
-    if (dtype == ITTS_T_F32) floats<VEC, float>(in, out);
-    else if (dtype == ITTS_T_BF16) floats<VEC, __bf16>(in, out);
-    else floats<VEC, _Float16>(in, out);
+__device__ __forceinline__ void floats_as(const Raw<E>& in, uint32_t c, uint32_t cols, int dtype, float (&out)[E]) {
+    if (dtype == ITTS_T_F32) floats<VEC, float>(in, c, cols, out);
+    else if (dtype == ITTS_T_BF16) floats<VEC, __bf16>(in, c, cols, out);
+    else floats<VEC, _Float16>(in, c, cols, out);
 }
 
 // Orders a wave's LDS accesses before and after it.
@@ -59,11 +59,11 @@ __global__ __launch_bounds__(1024) void rows_kernel(RowsArgs ra) {
         load_raw<VEC>(static_cast<const T*>(a.x) + r * a.x_stride, c, width(r), xr[i]);
         if constexpr (RES) load_raw<VEC>(static_cast<const T*>(a.residual) + r * a.residual_stride, c, width(r), rr[i]);
     };
-    auto hidden = [&](int i) {
-        floats<VEC, T>(xr[i], v[i]);
+    auto hidden = [&](int64_t r, uint32_t c, int i) {
+        floats<VEC, T>(xr[i], c, width(r), v[i]);
         if constexpr (RES) {
             float u[kElems];
-            floats<VEC, T>(rr[i], u);
+            floats<VEC, T>(rr[i], c, width(r), u);
 #pragma unroll
             for (int e = 0; e < kElems; ++e) v[i][e] = to_float(from_float<T>(v[i][e] + u[e]));
         }
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(1024) void rows_kernel(RowsArgs ra) {
                 weights();
             }
 #pragma unroll
-            for (int i = 0; i < CH; ++i) hidden(i);
+            for (int i = 0; i < CH; ++i) hidden(r, tid * kElems + i * step, i);
             if constexpr (NEXT) {
                 if (r0 + each < a.rows) begin(r + each);
             }
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(1024) void rows_kernel(RowsArgs ra) {
                 double sum = 0.0;
                 for (int i = 0; i < passes; ++i) {
                     fetch(r, tid * kElems + i * step, 0);
-                    hidden(0);
+                    hidden(r, tid * kElems + i * step, 0);
                     sum += quad_squares(v[0]) + quad_squares(v[0] + 4);
                 }
                 mine[tid] = sum;
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(1024) void rows_kernel(RowsArgs ra) {
             if (cols == 0 || c >= static_cast<uint32_t>(ra.kp)) return;  // (whole groups)
             if (h) store_row<VEC>(h, c, cols, v[i]);
             float w[kElems], code[kElems];
-            if (norm) floats_as<VEC>(wr[i], a.weight_dtype, w);
+            if (norm) floats_as<VEC>(wr[i], c, a.cols, a.weight_dtype, w);
             const float s = group_codes(v[i], w, norm, inv, a.group, (c & -static_cast<uint32_t>(a.group)) < cols, code);
             *reinterpret_cast<uint2*>(a.q + r * ra.kp + c) = make_uint2(four_codes(code), four_codes(code + 4));
             if ((c & (a.group - 1)) == 0) a.scales[r * (ra.kp >> ra.shift) + (c >> ra.shift)] = s;
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(1024) void rows_kernel(RowsArgs ra) {
                 const uint32_t c = tid * kElems + i * step;
                 fetch(r, c, 0);
                 if (norm) load_raw_as<VEC>(a.weight, c, a.cols, a.weight_dtype, wr[0]);
-                hidden(0);
+                hidden(r, c, 0);
                 codes(c, 0);
             }
         }
@@ -174,8 +174,9 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     const int64_t t = blockIdx.x, row = t / kb * kTileRows + r;
     Raw<kElems> raw;
     float v[kElems];
-    load_raw<VEC>(static_cast<const T*>(a.w) + row * a.stride, t % kb * kTileCols + 32 * b + 8 * j, row < a.n ? a.k : 0, raw);
-    floats<VEC, T>(raw, v);
+    const uint32_t col = static_cast<uint32_t>(t % kb) * kTileCols + 32 * b + 8 * j, cols = row < a.n ? a.k : 0;
+    load_raw<VEC>(static_cast<const T*>(a.w) + row * a.stride, col, cols, raw);
+    floats<VEC, T>(raw, col, cols, v);
     // the larger of max w / 7 and -min w / 8, or infinity where a value is not finite
     float mx = -INFINITY, mn = -INFINITY, bad = 0.0f;
 #pragma unroll
@@ -308,7 +309,8 @@ __device__ __forceinline__ void finish(const ProductArgs& a, int m, int n, float
     if (live) store_as(a.out, m * a.out_stride + col, a.dtype, v);
 }
 
-// The same for eight weight rows from n, a multiple of eight, at once.
+// The same for eight weight rows from n, a multiple of eight, at once.  Rows that are not 16-byte aligned are written in the
+// same pieces but for their ends (2048 x 10241 x 1280 to FP16 with a residual: 56 us; one by one 99; 10240: 53).
 template <class T, int N>
 __device__ __forceinline__ void finish_row(const ProductArgs& a, int m, int col, int cols, float (&v)[N]) {
     T* out = static_cast<T*>(a.out) + m * a.out_stride + col;
@@ -329,6 +331,20 @@ __device__ __forceinline__ void finish_row(const ProductArgs& a, int m, int col,
 #pragma unroll
             for (int i = 0; i < P; ++i) o.v[i] = from_float<T>(v[k * P + i]);
             reinterpret_cast<Piece*>(out)[k] = o;
+        }
+    } else if (col + N <= cols) {
+        constexpr int W = sizeof(Piece) / 4;
+#pragma unroll
+        for (int k = 0; k < N / P; ++k) {
+            Piece o;
+            if (res) {
+                const Piece r = __builtin_bit_cast(Piece, reinterpret_cast<const Loose<T, W>*>(res)[k]);
+#pragma unroll
+                for (int i = 0; i < P; ++i) v[k * P + i] += to_float(r.v[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < P; ++i) o.v[i] = from_float<T>(v[k * P + i]);
+            reinterpret_cast<Loose<T, W>*>(out)[k] = __builtin_bit_cast(Loose<T, W>, o);
         }
     } else {
 #pragma unroll
@@ -496,19 +512,19 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
                 if (r.weight) load_raw_as<false>(r.weight, p * 4, a.k, r.weight_dtype, g);
             }
         };
-        auto convert = [&](const Raw<4>& vr, const Raw<4>& gr, float (&v)[4], float (&g)[4]) {
+        auto convert = [&](int p, const Raw<4>& vr, const Raw<4>& gr, float (&v)[4], float (&g)[4]) {
             if (fa.vec) {
-                floats_as<true>(vr, r.dtype, v);
-                if (r.weight) floats_as<true>(gr, r.weight_dtype, g);
+                floats_as<true>(vr, p * 4, a.k, r.dtype, v);
+                if (r.weight) floats_as<true>(gr, p * 4, a.k, r.weight_dtype, g);
             } else {
-                floats_as<false>(vr, r.dtype, v);
-                if (r.weight) floats_as<false>(gr, r.weight_dtype, g);
+                floats_as<false>(vr, p * 4, a.k, r.dtype, v);
+                if (r.weight) floats_as<false>(gr, p * 4, a.k, r.weight_dtype, g);
             }
         };
         auto fetch = [&](int p, float (&v)[4], float (&g)[4]) {
             Raw<4> vr, gr;
             request(p, vr, gr);
-            convert(vr, gr, v, g);
+            convert(p, vr, gr, v, g);
         };
         auto norm = [&](int p, const float (&v)[4]) {
             const double s = pair64<1>(quad_squares(v), add64);
@@ -532,7 +548,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(FewArgs fa) {
             if (tid + i * T < quads) request(tid + i * T, x0[i], w0[i]);
         if (!active) return;
 #pragma unroll
-        for (int i = 0; i < KEEP; ++i) convert(x0[i], w0[i], v0[i], g0[i]);
+        for (int i = 0; i < KEEP; ++i) convert(tid + i * T, x0[i], w0[i], v0[i], g0[i]);
         if (r.weight) {
 #pragma unroll
             for (int i = 0; i < KEEP; ++i)
@@ -714,8 +730,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void batch_kernel(ProductArgs a) {
 // the two scales and a multiply-add a value in the vector units, and those add to the matrix instructions' time rather than
 // hide beside it: at 2048 x 10240 x 5120 in groups of 128 a block of 32 x 32 and a group costs about 300 cycles of the former
 // and 130 of the latter, and runs in 480 (161 us).  The outer product of scales as a matrix instruction of its own took 171 us,
-// the last block of a turn scaled beside the next turn's products 163 (and 174 became 247 in blocks of 128 x 128).  A workgroup owns 32 WM MT tokens x 32 WN NT weight rows.  WM x WN waves share a tile of codes staged through
-// LDS; weights go from memory to registers, in the order of the instruction's operand; the next turn's loads
+// the last block of a turn scaled beside the next turn's products 163 (and 174 became 247 in blocks of 128 x 128).
+// A workgroup owns 32 WM MT tokens x 32 WN NT weight rows.  WM x WN waves share a tile of codes staged through LDS; weights go from memory to registers, in the order of the instruction's operand; the next turn's loads
 // are under way while this one's are multiplied.  WK such groups of waves take every WK-th tile of columns and
 // add their sums through LDS in order.
 // v_mfma_i32_32x32x32_i8, not 16x16x64: the same operands give twice the products, and four waves

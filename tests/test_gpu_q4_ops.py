@@ -380,6 +380,56 @@ def test_autograd_sees_given_outputs_change(itts, ops):
     assert full._version == before + 1
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [5, 8, 67, 136, 1283])
+def test_rows_at_any_address(ops, cols, dtype):
+    """Rows that begin at each of eight places in 16 bytes, and at another one each: the bits of aligned
+    ones, and not an element around them changed."""
+    r = rng(cols, 5)
+    x, res = (tensor(r.standard_normal((21, cols)), dtype) for _ in range(2))
+    w = tensor(1 + 0.1 * r.standard_normal(cols), dtype)
+    pad = -(-cols // 8) * 8
+    want = ops.rmsnorm_q8(x, w, residual=res, values=True)
+    packed = ops.q4_pack(x, 32)
+    eight = ops.q8_quantize(tensor(r.standard_normal((40, 64))), 64)
+    columns = ops.q4_pack(tensor(r.standard_normal((cols, 64))), 64)
+    bias = tensor(r.standard_normal((40, cols)), dtype)
+    products = {rows: ops.q4_matmul(eight.q[:rows], eight.scales[:rows], columns, residual=bias[:rows], out_dtype=dtype) for rows in (3, 9, 40)}
+    full = ops.q4_unpack(packed, dtype)
+    for at in range(8):
+        for stride in (pad + 16, pad + 17):
+
+            def place(t=None, rows=21):
+                whole = torch.full((rows + 1, stride), 7.0, dtype=dtype, device="cuda")
+                part = torch.as_strided(whole, (rows, cols), (stride, 1), at)
+                if t is not None:
+                    part.copy_(t)
+                return whole, part
+
+            def only(whole, part, value):
+                assert torch.equal(part, value), (at, stride)
+                part.fill_(7.0)
+                assert torch.equal(whole, torch.full_like(whole, 7.0)), (at, stride)
+
+            px, pr, (wh, ph), (wv, pv) = place(x)[1], place(res)[1], place(), place()
+            weight = torch.as_strided(place(w.expand(21, cols))[0], (cols,), (1,), at)
+            got = ops.rmsnorm_q8(px, weight, residual=pr, h=ph, values=pv)
+            assert torch.equal(got.q, want.q) and torch.equal(got.scales, want.scales)
+            only(wh, ph, want.h)
+            only(wv, pv, want.values)
+            again = ops.q4_pack(px, 32)
+            assert torch.equal(again.packed, packed.packed) and torch.equal(again.scales, packed.scales)
+            wo, po = place()
+            ops.q4_unpack(packed, dtype, out=po)
+            only(wo, po, full)
+            for rows, product in products.items():
+                wo, po = place(rows=rows)
+                ops.q4_matmul(eight.q[:rows], eight.scales[:rows], columns, residual=place(bias[:rows], rows)[1], out_dtype=dtype, out=po)
+                only(wo, po, product)
+            one = ops.q4_linear(px[:1], ops.Q4Weight(*ops.q4_pack(x, 128)), norm_weight=weight)
+            assert torch.equal(one, ops.q4_linear(x[:1], ops.q4_pack(x, 128), norm_weight=w))
+
+
 # ------------------------------------------------------------------ a layer's run of them
 def layer(ops, x, r_in, ws, nws, dtype):
     a = ops.rmsnorm_q8(x, nws[0], 1e-6, residual=r_in)
