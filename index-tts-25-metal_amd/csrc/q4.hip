@@ -728,12 +728,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void batch_kernel(ProductArgs a) {
 
 // More than 16 tokens: bound by the scaling.  Every group's 32-bit sums take a conversion, the product of
 // the two scales and a multiply-add a value in the vector units, and those add to the matrix instructions' time rather than
-// hide beside it: at 2048 x 10240 x 5120 in groups of 128 a block of 32 x 32 and a group costs about 300 cycles of the former
-// and 130 of the latter, and runs in 480 (161 us).  The outer product of scales as a matrix instruction of its own took 171 us,
+// hide beside it: at 2048 x 10240 x 5120 in groups of 128 a block of 32 x 32 and a group costs about 270 cycles of the former
+// and 140 of the latter, and runs in 430 (161 us).  The outer product of scales as a matrix instruction of its own took 171 us,
 // the last block of a turn scaled beside the next turn's products 163 (and 174 became 247 in blocks of 128 x 128).
-// A workgroup owns 32 WM MT tokens x 32 WN NT weight rows.  WM x WN waves share a tile of codes staged through LDS; weights go from memory to registers, in the order of the instruction's operand; the next turn's loads
-// are under way while this one's are multiplied.  WK such groups of waves take every WK-th tile of columns and
-// add their sums through LDS in order.
+// A workgroup owns 32 WM MT tokens x 32 WN NT weight rows.  WM x WN waves share a tile of codes staged through LDS;
+// weights go from memory to registers, in the order of the instruction's operand; the next turn's loads are under way while
+// this one's are multiplied.  WK such groups of waves take every WK-th tile of columns and add their sums through LDS in order.
 // v_mfma_i32_32x32x32_i8, not 16x16x64: the same operands give twice the products, and four waves
 // of a SIMD ran them at 35 cycles each against 29 for half the work.
 // The instruction takes 16 consecutive columns from each half of the wave: 64 p + 32 b + 16 h + 0..15 for
