@@ -14,7 +14,6 @@ row r at columns 64 p + 8 j + i (low half) and 64 p + 32 + 8 j + i (high half), 
 tiles first; scales bf16 [tile row][tile][16 rows][128 / group]; rows and columns behind the matrix are zero.
 Codes of activations are int8 [rows][columns up to a multiple of 128], their scales float32.
 """
-import functools
 import math
 import sys
 from pathlib import Path
@@ -197,9 +196,8 @@ def prepare(case, seed):
 
 
 # ------------------------------------------------------------------ one pass
-@functools.lru_cache(maxsize=None)
 def operators():
-    """The framework's operators, imported once as a program does."""
+    """The framework's operators."""
     at = str(Path.cwd() / "index-tts-25-metal_amd")
     if at not in sys.path:
         sys.path.insert(0, at)
