@@ -842,6 +842,7 @@ struct Engine {
     void ensure_prefill(int P) {
         if (P <= pcap) return;
         const int cap = std::max(P, 256);
+        pcap = 0;  // until all are there: after a failed allocation the next prefill makes them again
         X.alloc(static_cast<size_t>(cap) * kD);
         QKV.alloc(static_cast<size_t>(cap) * kQkvN);
         Qp.alloc(static_cast<size_t>(cap) * kQ);
@@ -850,14 +851,13 @@ struct Engine {
             code_scales.alloc(static_cast<size_t>(cap) * (kF / kQ4Group));
             ATTf.alloc(static_cast<size_t>(cap) * kQ);
             FFf.alloc(static_cast<size_t>(cap) * kF);
-            pcap = cap;
-            return;
+        } else {
+            Xn.alloc(split_elems(cap, kD));
+            ATT.alloc(split_elems(cap, kQ));
+            FF.alloc(split_elems(cap, kF));
+            for (auto* b : {&Xn, &ATT, &FF}) QWEN_CHECK(hipMemsetAsync(b->p, 0, b->n * 2, stream));  // padding rows: finite, whatever the memory held
+            if (!ws.p) ws.alloc(kGemmWsFloats);
         }
-        Xn.alloc(split_elems(cap, kD));
-        ATT.alloc(split_elems(cap, kQ));
-        FF.alloc(split_elems(cap, kF));
-        for (auto* b : {&Xn, &ATT, &FF}) QWEN_CHECK(hipMemsetAsync(b->p, 0, b->n * 2, stream));  // padding rows: finite, whatever the memory held
-        if (!ws.p) ws.alloc(kGemmWsFloats);
         pcap = cap;
     }
 
