@@ -34,7 +34,7 @@ typedef struct itts_qwen itts_qwen;
 
 typedef struct {
     uint32_t layers; /* decoder layers; 0 -> 28, the reference's (qwen.cpp:8) */
-    uint32_t flags;  /* 0 or ITTS_QWEN_W4, ITTS_QWEN_W4_HEAD; the other bits are reserved, 0 */
+    uint32_t flags;  /* 0 or ITTS_QWEN_W4, ITTS_QWEN_W4_HEAD; the other bits are reserved and refused */
 } itts_qwen_config;
 
 /* QwenDecoder::QwenDecoder (qwen.cpp:5-15): the tensors by their reference names

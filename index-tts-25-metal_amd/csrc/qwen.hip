@@ -727,6 +727,7 @@ struct Engine {
     float* Vc(int l) const { return kv.p + static_cast<size_t>(2 * l + 1) * kKVH * kCap * kHd; }
 
     void create(const std::unordered_map<std::string, Tensor>& t, uint32_t nlayers, uint32_t flags) {
+        if (flags & ~(ITTS_QWEN_W4 | ITTS_QWEN_W4_HEAD)) throw std::invalid_argument("Unknown Qwen flag");
         layers = nlayers ? static_cast<int>(nlayers) : 28;
         q4_layers = flags & ITTS_QWEN_W4;
         q4_head = flags & ITTS_QWEN_W4_HEAD;
