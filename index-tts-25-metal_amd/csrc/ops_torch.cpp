@@ -11,6 +11,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPFunctions.h>
@@ -152,6 +153,9 @@ public:
         if (t->is_neg()) no("a negated view: resolve_neg() it first");
         if (t->requires_grad() && c10::GradMode::is_enabled())
             no("these operators have no gradients: detach the tensors, or call under torch.no_grad()");
+        // (a dual tensor of forward mode: its tangent would be lost)
+        if (t->_fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+            no("these operators have no gradients: unpack_dual() the tensors of forward mode");
     }
     void enter() {
         also(&first_);

@@ -12,7 +12,7 @@ float16 with unit column stride; `group` is 32, 64 or 128 columns.  Calls run on
 the tensors' device and return without waiting for it; none keeps anything between calls, and all
 may be captured into a graph.  Outputs that are not given are made.  Arguments that do not fit
 raise InvalidArgument.  There are no gradients (tensors that require them are refused unless under
-no_grad) and there is no CPU path.
+no_grad, and so are forward mode's dual tensors) and there is no CPU path.
 
 The library has to run on the HIP runtime that torch brings, whose streams it is given: import torch (or
 this module) before itts_gpt, else two runtimes are loaded and this import fails.
