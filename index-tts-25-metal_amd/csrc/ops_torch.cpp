@@ -5,6 +5,7 @@
 // they stand here.  Host code only: it hands addresses to the C ABI.
 #include <Python.h>
 
+#include <initializer_list>
 #include <sstream>
 #include <stdexcept>
 #include <string>
@@ -186,11 +187,14 @@ void done(int status) {
 }
 void* at_of(const Tensor* t) { return t ? t->data_ptr() : nullptr; }
 
-// A given output: autograd has to see that its values change.
-const Tensor& written(const Tensor& t) {
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-    else if (!c10::InferenceMode::is_enabled()) no("an output made in inference mode, outside of it");
+// A given output, before the call and after it: autograd has to see that its values change, by a call that is not refused.
+const Tensor& writable(const Tensor& t) {
+    if (t.is_inference() && !c10::InferenceMode::is_enabled()) no("an output made in inference mode, outside of it");
     return t;
+}
+void written(std::initializer_list<const Tensor*> given) {
+    for (const Tensor* t : given)
+        if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
 Tensor make(at::IntArrayRef sizes, const Tensor& like_, at::ScalarType type) { return at::detail::empty_cuda(sizes, type, like_.device(), std::nullopt); }
@@ -211,7 +215,7 @@ Codes codes(const Tensor& x, int64_t rows, int64_t cols, int64_t group, const Te
                    !scales->is_contiguous()))
         no("scales: contiguous float32 [", rows, ", ", kp / group, "] is wanted");
     on();
-    return {q ? written(*q) : make({rows, kp}, x, at::kChar), scales ? written(*scales) : make({rows, kp / group}, x, at::kFloat)};
+    return {q ? writable(*q) : make({rows, kp}, x, at::kChar), scales ? writable(*scales) : make({rows, kp / group}, x, at::kFloat)};
 }
 
 // (x, weight or None, eps, residual, group, h, q, scales, values) -> (h, q, scales, values)
@@ -234,15 +238,16 @@ PyObject* rows_to_codes(PyObject* const* a, bool norm) {
     const bool values = a[8] == Py_True;
     if (!values && a[8] != Py_False) v_in = optional(a[8], "values");
     if (v_in) vs = like(*v_in, x.scalar_type(), m.rows, m.cols, "values");
+    const Tensor *q_in = optional(a[6], "q"), *s_in = optional(a[7], "scales");
     On on(x);
-    const Codes c = codes(x, m.rows, m.cols, group, optional(a[6], "q"), optional(a[7], "scales"), [&] {
-        for (const Tensor* t : {w, residual, h_in, v_in, optional(a[6], "q"), optional(a[7], "scales")}) on.also(t);
+    const Codes c = codes(x, m.rows, m.cols, group, q_in, s_in, [&] {
+        for (const Tensor* t : {w, residual, h_in, v_in, q_in, s_in}) on.also(t);
         on.enter();
     });
     Tensor h, v;
-    if (h_in) h = written(*h_in);
+    if (h_in) h = writable(*h_in);
     else if (residual) h = make({m.rows, m.cols}, x, x.scalar_type());
-    if (v_in) v = written(*v_in);
+    if (v_in) v = writable(*v_in);
     else if (values) v = make({m.rows, m.cols}, x, x.scalar_type());
     void* const hp = h.defined() ? h.data_ptr() : nullptr;
     void* const vp = v.defined() ? v.data_ptr() : nullptr;
@@ -252,6 +257,7 @@ PyObject* rows_to_codes(PyObject* const* a, bool norm) {
     else
         done(itts_q8_quantize(x.data_ptr(), m.stride, m.kind, m.rows, m.cols, static_cast<int32_t>(group), vp, vs, static_cast<int8_t*>(c.q.data_ptr()),
                               static_cast<float*>(c.scales.data_ptr()), on.stream()));
+    written({h_in, v_in, q_in, s_in});
     PyObject* out = PyTuple_New(norm ? 4 : 3);
     if (!out) throw python_error();
     int i = 0;
@@ -303,8 +309,9 @@ PyObject* unpack(PyObject* const* a) {
     on.also(w.scales);
     on.also(given);
     on.enter();
-    const Tensor out = given ? written(*given) : make({w.n, w.k}, *w.packed, type_of(kind));
+    const Tensor out = given ? writable(*given) : make({w.n, w.k}, *w.packed, type_of(kind));
     done(itts_q4_unpack(w.packed->data_ptr(), w.scales->data_ptr(), w.n, w.k, static_cast<int32_t>(w.group), kind, out.data_ptr(), os, on.stream()));
+    written({given});
     return wrap(out);
 }
 
@@ -335,7 +342,7 @@ struct Product {
     void on(const On& o, const Weight& w) const {
         for (const Tensor* t : {w.packed, w.scales, bias, residual, given}) o.also(t);
     }
-    Tensor out(int64_t rows, const Tensor& x) const { return given ? written(*given) : make({rows, cols}, x, type_of(kind)); }
+    Tensor out(int64_t rows, const Tensor& x) const { return given ? writable(*given) : make({rows, cols}, x, type_of(kind)); }
     const float* bias_at() const { return static_cast<const float*>(at_of(bias)); }
     uint32_t flags() const { return swiglu ? ITTS_Q4_SWIGLU : 0u; }
 };
@@ -358,6 +365,7 @@ PyObject* matmul(PyObject* const* a) {
     const Tensor out = p.out(rows, q);
     done(itts_q4_matmul(static_cast<const int8_t*>(q.data_ptr()), static_cast<const float*>(s.data_ptr()), rows, w.packed->data_ptr(), w.scales->data_ptr(), w.n,
                         w.k, static_cast<int32_t>(w.group), p.bias_at(), at_of(p.residual), p.rs, p.flags(), p.kind, out.data_ptr(), p.os, on.stream()));
+    written({p.given});
     return wrap(out);
 }
 
@@ -381,6 +389,7 @@ PyObject* linear(PyObject* const* a) {
     done(itts_q4_linear(x.data_ptr(), m.stride, m.kind, m.rows, at_of(nw), wkind, static_cast<float>(eps), w.packed->data_ptr(), w.scales->data_ptr(), w.n, w.k,
                         static_cast<int32_t>(w.group), p.bias_at(), at_of(p.residual), p.rs, p.flags(), p.kind, out.data_ptr(), p.os,
                         need ? work.data_ptr() : nullptr, need, on.stream()));
+    written({p.given});
     return wrap(out);
 }
 
