@@ -1085,7 +1085,8 @@ hipError_t launch_fused(const FewArgs& given, hipStream_t s) {
     return by_group(a.p.group, [&](auto g) { return few_rows<decltype(g)::value, kFromRow>(a, s); });
 }
 
-hipError_t launch_merged(const FewArgs& a, hipStream_t s) { return few_rows<128, kFromParts>(a, s); }
+// (turns of two tiles: those of the decoder's 16 heads, two a wave)
+hipError_t launch_merged(const FewArgs& a, hipStream_t s) { return launch_few<128, 1, 2, kFromParts>(a, std::min(pad_cols(a.p.k) / kTileCols, kFewWaves), s); }
 
 hipError_t launch_linear(const ProductArgs& product, const NormArgs& rows, hipStream_t s) {
     if (product.rows == 0) return hipSuccess;
