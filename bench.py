@@ -116,33 +116,38 @@ def batch8_inputs(it, dec):
     return prefixes, opts
 
 
-QWEN_WEIGHT_BYTES = 28 * 15_728_640 * 4 + 151_936 * 1024 * 4 + (28 * 2304 + 1024) * 4  # slab, tied embedding, norms
+QWEN_MATRIX_CELLS = 28 * 15_728_640 + 151_936 * 1024  # the layers' matrices and the tied embedding
+QWEN_NORM_BYTES = (28 * 2304 + 1024) * 4
+QWEN_CELL_BYTES = {32: 4, 4: 0.5 + 2 / 128}           # 4 bits: a BF16 scale per 128 columns
 QWEN_KV_BYTES_PER_ROW = 28 * 2 * 8 * 128 * 4                                        # K and V of one row, all layers
 
 
-def qwen_step_bytes(rows: int) -> float:
+def qwen_step_bytes(rows: int, bits: int) -> float:
     """Algorithmic HBM bytes of one Qwen decode step with `rows` cache rows after it: every
     weight byte once, the cache rows' K and V, the 151936 logits written."""
-    return QWEN_WEIGHT_BYTES + QWEN_KV_BYTES_PER_ROW * rows + 151_936 * 4
+    return QWEN_MATRIX_CELLS * QWEN_CELL_BYTES[bits] + QWEN_NORM_BYTES + QWEN_KV_BYTES_PER_ROW * rows + 151_936 * 4
 
 
-def qwen_workload(it):
-    """The Qwen3-0.6B emotion-text decoder (src/qwen.cpp), 28 layers, synthetic weights: a
-    64-id prompt, greedy generation of 256 ids (random weights reach no EOS, so every call runs
-    to the maximum), whole-call tokens/s; prefill time and the decode step's HIP-event time at
-    64 + 128 cache rows."""
-    q = it.QwenDecoder(it.make_synthetic_qwen_weights(seed=1))
+def qwen_workload(it, bits=32, lengths=()):
+    """The Qwen3-0.6B emotion-text decoder (src/qwen.cpp), 28 layers, synthetic weights in 32 or
+    4 bits: a 64-id prompt, greedy generation of 256 ids (random weights reach no EOS, so every
+    call runs to the maximum), whole-call tokens/s; prefill time and the decode step's HIP-event
+    time at 64 + 128 cache rows, and at others: (prompt, cache rows) in `lengths`."""
+    q = it.QwenDecoder(it.make_synthetic_qwen_weights(seed=1), weight_bits=bits)
     prompt = [int(x) for x in np.random.default_rng(12).integers(0, 151936, 64)]
     q.generate_tokens(prompt, 32)
     r, times = timed(lambda: q.generate_tokens(prompt, 256), 2)
     prefill_ms, step_us = q.bench(64, 64 + 128, 100)
+    more = [q.bench(p, c, 100) for p, c in lengths]
     q.close()
     rows = 64 + 128 + 50  # the mean cache length over the 100 timed steps, plus the new row
-    gbs = qwen_step_bytes(rows) / (step_us * 1e-6) / 1e9
+    gbs = qwen_step_bytes(rows, bits) / (step_us * 1e-6) / 1e9
     return {"prompt": 64, "generated": len(r[0]), "reached_eos": r[1], "seconds": round(min(times), 4),
             "tokens_per_s": round(len(r[0]) / min(times), 2), "prefill_ms_64": round(prefill_ms, 3),
             "step_us_at_192_rows": round(step_us, 2), "step_algorithmic_GBps": round(gbs, 1),
-            "step_hbm_frac": round(gbs / HBM_PEAK_GBS, 4)}
+            "step_hbm_frac": round(gbs / HBM_PEAK_GBS, 4),
+            **{f"prefill_ms_{p}": round(ms, 3) for (p, _), (ms, _) in zip(lengths, more)},
+            **{f"step_us_at_{c}_rows": round(us, 2) for (_, c), (_, us) in zip(lengths, more)}}
 
 
 def extras(it, dec, weights):
@@ -249,7 +254,7 @@ def main() -> int:
     ap.add_argument("--no-extras", action="store_true")
     ap.add_argument("--kernel-only", default=None, help="time one kernel kind only (for profiler runs); 'codec': a 600-code codec decode; 'beam3': the beam-3 workload; "
                          "'batch8' / 'batch8_bf16': the 8-sequence workload; "
-                         "'prefill': the 155-row prefill; 'qwen': the Qwen3 emotion-text decoder")
+                         "'prefill': the 155-row prefill; 'qwen' / 'qwen_w4': the Qwen3 emotion-text decoder with FP32 / 4-bit weights")
     ap.add_argument("--iters", type=int, default=240)
     ap.add_argument("--kernel-batch", type=int, default=1, help="sequences per launch for --kernel-only")
     args = ap.parse_args()
@@ -300,10 +305,11 @@ def main() -> int:
                           "ms_per_step": round(tm["decode_ms"] / max(1, tm["decode_steps"] - 1), 4),
                           "prefill_ms": round(tm["prefill_ms"], 3)}), flush=True)
         return 0
-    if args.kernel_only == "qwen":
-        # the extras' Qwen workload alone (64-id prompt, 256 greedy ids, 28 layers), for profilers
+    if args.kernel_only in ("qwen", "qwen_w4"):
+        # the extras' Qwen workload alone (64-id prompt, 256 greedy ids, 28 layers), for profilers; and longer prompts
         dec.close()
-        print(json.dumps({"kernel": "qwen", **qwen_workload(it)}), flush=True)
+        bits = 4 if args.kernel_only == "qwen_w4" else 32
+        print(json.dumps({"kernel": args.kernel_only, **qwen_workload(it, bits, ((512, 1000), (2048, 2000)))}), flush=True)
         return 0
     if args.kernel_only == "codec":
         codec = it.EnhancedCodec(it.make_synthetic_codec_weights(seed=0))
