@@ -90,7 +90,9 @@ int itts_q4_unpack(const void* packed, const void* scales, int64_t n, int64_t k,
 /* out[m][j] = sum over k of x[m][k] w[j][k], x and w being what the codes q, qscales [rows] and
  * packed, scales [n] stand for; + bias[j] (F32 [n] or NULL); SwiGLU with ITTS_Q4_SWIGLU (n even);
  * + residual[m][j] (`dtype`, or NULL); rounded to `dtype` once.  out may be residual itself.
- * The codes' products are summed exactly within a group, the groups in FP32. */
+ * The codes' products are summed exactly within a group, the groups in FP32.  A group's two scales are
+ * multiplied in FP32 first: where their product leaves its range, so does what the group adds: infinite or NaN
+ * above it, with fewer bits where the product is under 2e-37. */
 int itts_q4_matmul(const int8_t* q, const float* qscales, int64_t rows, const void* packed, const void* scales, int64_t n, int64_t k,
                    int32_t group, const float* bias, const void* residual, int64_t residual_stride, uint32_t flags, int32_t dtype,
                    void* out, int64_t out_stride, void* stream);

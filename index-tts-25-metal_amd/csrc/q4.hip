@@ -31,9 +31,13 @@ __device__ __forceinline__ void wave_sync() {
 }
 
 // ------------------------------------------------------------------ rows to 8 bits
-// Bound by memory: every element is read once.  A team of waves owns a row and keeps it in registers between the
-// two passes, CH runs of eight columns a lane; the norm's weights are requested with the row.  CH = 0: rows
-// longer than that, by 1024 threads, which read h (or x) again.
+// Every element is read once: a team of waves owns a row and keeps it in registers between the two passes, CH runs of eight
+// columns a lane; the norm's weights are requested with the row.  CH = 0: rows longer than that, by 1024 threads,
+// which read h (or x) again.
+// What bounds it, on inputs that come from memory: the quantisation of wide aligned rows, memory (4096 x 4096 FP32 16.4 us, a copy's
+// rate).  With the norm, the chain of each row, its sums through two barriers and then its codes, which only CH = 1 overlaps with
+// the next row's loads: 8192 x 5120 BF16 67 us without and 80 with a residual, where a copy of the same bytes takes 25 and 57; 84 MB of
+// `values` beside that, 16 us for a copy, cost 9.  8192 x 1280 FP16 20 us, 2048 x 4096 FP32 15.
 struct RowsArgs {
     NormArgs a;
     int kp, waves, shift;  // padded columns; waves of a team; log2 of the group
@@ -310,7 +314,7 @@ __device__ __forceinline__ void finish(const ProductArgs& a, int m, int n, float
 }
 
 // The same for eight weight rows from n, a multiple of eight, at once.  Rows that are not 16-byte aligned are written in the
-// same pieces but for their ends (2048 x 10241 x 1280 to FP16 with a residual: 56 us; one by one 99; 10240: 53).
+// same pieces but for their ends (2048 x 10241 x 1280 to FP16 with a residual: 56 us; one by one 96; 10240: 52).
 template <class T, int N>
 __device__ __forceinline__ void finish_row(const ProductArgs& a, int m, int col, int cols, float (&v)[N]) {
     T* out = static_cast<T*>(a.out) + m * a.out_stride + col;
@@ -726,11 +730,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void batch_kernel(ProductArgs a) {
     }
 }
 
-// More than 16 tokens: bound by the scaling.  Every group's 32-bit sums take a conversion, the product of
-// the two scales and a multiply-add a value in the vector units, and those add to the matrix instructions' time rather than
-// hide beside it: at 2048 x 10240 x 5120 in groups of 128 a block of 32 x 32 and a group costs about 270 cycles of the former
-// and 140 of the latter, and runs in 430 (161 us).  The outer product of scales as a matrix instruction of its own took 171 us,
-// the last block of a turn scaled beside the next turn's products 163 (and 174 became 247 in blocks of 128 x 128).
+// More than 16 tokens: bound by the scaling, in this schedule.  Every group's 32-bit sums take a conversion, the product of
+// the two scales and a multiply-add a value in the vector units: at 2048 x 10240 x 5120 in groups of 128 a block of 32 x 32
+// and a group costs about 270 cycles of those and 140 of matrix instructions, and runs in 430 (162 us; SwiGLU 166, in groups
+// of 64 216, of 32 312), as if the two came one after the other.  The machine does not ask for that: 32 v_fma_f32 beside four
+// v_mfma_i32_32x32x32_i8 take 191 cycles where apart they take 142 and 139.  The outer product of scales as a matrix
+// instruction of its own took 171 us, the last block of a turn scaled beside the next turn's products 163 (and 174 became
+// 247 in blocks of 128 x 128).
 // A workgroup owns 32 WM MT tokens x 32 WN NT weight rows.  WM x WN waves share a tile of codes staged through LDS;
 // weights go from memory to registers, in the order of the instruction's operand; the next turn's loads are under way while
 // this one's are multiplied.  WK such groups of waves take every WK-th tile of columns and add their sums through LDS in order.
@@ -990,8 +996,12 @@ hipError_t launch_rows(const NormArgs& a, hipStream_t s) {
 }
 
 namespace {
-// Matrices of so many rows take four tile rows a workgroup, which then reads the codes once for the four (16 rows x
-// 16384 x 8192: 15.2 us against 18.9; x 10240 x 5120: 9.5 against 10.4, but 8 rows 9.0 against 8.6).
+// Matrices of so many rows take four tile rows a workgroup, which then reads the codes once for the four and has more loads
+// under way; fewer rows leave too few workgroups for that.  Measured (us with one and with four tile rows):
+//   1 row: 16384 x 1024 3.9 4.3; 32768 x 512 4.1 4.4, x 1024 6.0 5.5, x 2048 8.1 8.0, x 5120 16.3 16.8; 151936 x 512 10.6 8.8,
+//     x 1024 18.8 14.2, x 2048 26.2 26.6, x 5120 60.1 60.7; 4 rows: four against one within 3% of that
+//   5 rows: 10240 x 1024 4.0 4.3, x 5120 8.5 8.3; 16384 x 1024 4.3 4.6, x 5120 10.7 9.4, x 8192 14.9 14.8; 65536 x 5120 35 28
+//   16 rows: 8192 x 5120 8.0 8.8; 10240 x 1024 4.1 4.5, x 5120 10.2 9.0; 16384 x 1024 4.6 4.7, x 5120 13.3 9.8, x 8192 19.0 14.5
 constexpr int kFewWide = 32768, kBatchWide = 16384;
 
 // Tiles of columns that a wave takes in a turn, of `each` in all: those that leave the fewest of its last turn

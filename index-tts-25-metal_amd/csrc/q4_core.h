@@ -64,8 +64,9 @@ __device__ __forceinline__ double add64(double a, double b) { return a + b; }
 __device__ __forceinline__ double max64(double a, double b) { return a > b || a != a ? a : b; }
 
 // ------------------------------------------------------------------ a row's squares
-// One order for every kernel: four neighbours one after the other, two such sums; of these eight-column sums every
-// 64th one after the other, then pairs of those.
+// One order for every kernel that keeps a row in registers: four neighbours one after the other, two such sums; of these
+// eight-column sums every 64th one after the other, then pairs of those.  (Rows of more than 32768 columns, which only one
+// kernel takes, are added a thread's passes first.)
 __device__ __forceinline__ double quad_squares(const float* v) {
     double s = static_cast<double>(v[0]) * static_cast<double>(v[0]);
 #pragma unroll
@@ -131,8 +132,8 @@ struct __attribute__((packed, aligned(sizeof(T)))) Loose {
 // E elements from column c of a row of `cols`, as they lie in memory (0 behind the row's end): loads alone, so
 // that several rows' are under way at once.  VEC: the row is 16-byte aligned and a multiple of eight columns long;
 // others'
-// elements come one by one only in the piece that the row's end cuts.  (All of them one by one: norm of 4096 x 5121 BF16
-// with a residual 106 us, now 64; packing and unpacking 16384 x 5121 115 and 180, now 69 and 78.)
+// elements come one by one only in the piece that the row's end cuts.  (All of them one by one, inputs from memory: norm of
+// 4096 x 5121 BF16 with a residual 132 us, so 80; packing and unpacking 16384 x 5121 139 and 202, so 75 and 88.)
 template <int E>
 struct Raw {
     uint32_t w[E];  // four bytes an element, or (two-byte types, whole pieces) two elements a word

@@ -27,7 +27,7 @@
 // captured once as a hipGraph; token, cache length and count live in device QState, so
 // generate() replays it with no per-token host work and polls a flag every 16 tokens.
 // With ITTS_QWEN_W4 the layers' matrices (ITTS_QWEN_W4_HEAD: the head's too) are held in 4 bits with a scale per 128
-// columns (q4.h; 0.24 GB instead of 1.76, 82 MB instead of 622) and the GEMVs become launch_fused: RMSNorm, the
+// columns (q4.h; 0.23 GB instead of 1.76, 80 MB instead of 622) and the GEMVs become launch_fused: RMSNorm, the
 // row's 8-bit codes and the product in one launch each.  The prefill norms rows to 8-bit codes and multiplies
 // those.  Embedding rows, norms, attention and the cache stay in FP32.
 // Prefill (P ids): embedding rows, RMSNorm rows, split-BF16 GEMMs of prefill.hip (store, residual
