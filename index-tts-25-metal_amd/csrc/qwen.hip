@@ -627,10 +627,14 @@ __global__ __launch_bounds__(64 * kAttnWaves) void q_causal_attn_kernel(QCausalA
     }
 }
 
+// (An error that is thrown is taken from the runtime too, or the next launch's check would find it again.)
 #define QWEN_CHECK(x)                                                                                        \
     do {                                                                                                     \
         const hipError_t e_ = (x);                                                                           \
-        if (e_ != hipSuccess) throw std::runtime_error(std::string("HIP error ") + hipGetErrorString(e_) + " in " #x); \
+        if (e_ != hipSuccess) {                                                                              \
+            (void)hipGetLastError();                                                                         \
+            throw std::runtime_error(std::string("HIP error ") + hipGetErrorString(e_) + " in " #x);         \
+        }                                                                                                    \
     } while (0)
 
 template <class T>

@@ -1,6 +1,7 @@
 """A prefill whose larger buffers cannot be had leaves a decoder that makes them again, or says so, and never
 launches on buffers that are gone.  On the CPU: a stand-in for the HIP runtime, loaded ahead of it, counts
-allocations and launches, refuses allocations when told to, and runs nothing."""
+allocations and launches, refuses allocations when told to, and runs nothing.  As the runtime does, it keeps the
+thread's last error until it is asked for, which is how launches are checked."""
 import shutil
 import subprocess
 import sys
@@ -18,12 +19,10 @@ STAND_IN = r"""
 #include <cstdlib>
 struct Dim { uint32_t x, y, z; };
 extern "C" {
-int allocations = 0, launches = 0, refuse_from = 0;  // refuse_from: the first allocation that fails, 0 for none
+int allocations = 0, launches = 0, refuse_from = 0, last = 0;  // refuse_from: the first allocation that fails, 0 for none
 int hipMalloc(void** p, size_t n) {
-    *p = nullptr;
-    if (++allocations >= refuse_from && refuse_from) return 2;
-    *p = std::malloc(n);
-    return *p ? 0 : 2;
+    *p = ++allocations >= refuse_from && refuse_from ? nullptr : std::malloc(n);
+    return *p ? 0 : (last = 2);
 }
 int hipFree(void* p) { std::free(p); return 0; }
 int hipHostMalloc(void** p, size_t n, unsigned) { *p = std::calloc(1, n); return 0; }
@@ -42,7 +41,11 @@ int hipEventRecord(void*, void*) { return 0; }
 int hipEventSynchronize(void*) { return 0; }
 int hipGetDevice(int* d) { *d = 0; return 0; }
 int hipDeviceGetAttribute(int* v, int, int) { *v = 256; return 0; }
-int hipGetLastError() { return 0; }
+int hipGetLastError() {
+    const int e = last;
+    last = 0;
+    return e;
+}
 int __hipPushCallConfiguration(Dim, Dim, size_t, void*) { return 0; }
 int __hipPopCallConfiguration(Dim* g, Dim* b, size_t* l, void** s) {
     *g = *b = Dim{1, 1, 1};
